@@ -14,7 +14,7 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float float2_u __attribute__((ext_vector_type(2), aligned(4)));  // 8-byte load with dword alignment
 typedef unsigned short ushort_u __attribute__((aligned(1)));             // 2-byte load with byte alignment
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));                 // a channel pair: v_pk_mul_f32 / v_pk_add_f32
+typedef float f32x2 __attribute__((ext_vector_type(2)));                 // a channel pair
 
 // ------------------------------------------------------------------------------------------------
 // Shared per-voxel gate (projection, occlusion test against the synthetic depth, bilinear footprint,
@@ -221,7 +221,7 @@ __device__ __forceinline__ half8 low_tap(const Low8& a00, const Low8& a01, const
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const float val = madd2<FMA>(Y.l0, madd2<FMA>(X.l0, low_at(a00, k), X.l1, low_at(a01, k)), Y.l1, madd2<FMA>(X.l0, low_at(a10, k), X.l1, low_at(a11, k)));
-    o[k] = (_Float16)val;
+    o[k] = half_of(val);
   }
   return o;
 }
@@ -237,7 +237,7 @@ __device__ __noinline__ half8 low_tap_at(const float* __restrict__ low, int w, i
 
 // One surviving voxel: blend its channel row with the bilinear sample of the feature image (or of the virtual up-sampled
 // low-res map).  `lanes` lanes (gl = 0..lanes-1) share the row in 16-byte pieces.
-// packed forms of madd2 (two channels per instruction: v_pk_fma_f32 / v_pk_mul_f32 + v_pk_add_f32)
+// madd2 of a channel pair
 template <int FMA>
 __device__ __forceinline__ f32x2 pk_madd2(float a, f32x2 x, float b, f32x2 y) {
   if constexpr ((FMA & 1) != 0) {
@@ -273,8 +273,8 @@ __device__ __forceinline__ void feature_voxel(const AppArgs& Aa, const MapConsts
     } else {
       av = *reinterpret_cast<const half8*>(A + ch * 8);
     }
-    // two channels per instruction (v_pk_mul_f32 / v_pk_add_f32: the same multiplications and additions in the same order, element
-    // by element -- no contraction): this loop is the instruction count of the row update, which is issue-bound as a guest of the
+    // two channels at a time (the same multiplications and additions in the same order, element by element -- no contraction; the
+    // build has no packed float32 instructions, see the Makefile): this loop is the instruction count of the row update, which is issue-bound as a guest of the
     // sphere-trace launch and, from a low-res map, on its own
     half8 o;
     const float ux = 1.0f - wx, uy = 1.0f - wy;
@@ -302,8 +302,8 @@ __device__ __forceinline__ void feature_voxel(const AppArgs& Aa, const MapConsts
       const f32x2 old = {(float)av[k], (float)av[k + 1]};
       const f32x2 num = pk_madd2<FMA>(old, Wv, a, wm);
       const f32x2 An = DIV ? num / (Wv + wm) : num * inv;
-      o[k] = (_Float16)An.x;
-      o[k + 1] = (_Float16)An.y;
+      o[k] = half_of(An.x);
+      o[k + 1] = half_of(An.y);
     }
     *reinterpret_cast<half8*>(A + ch * 8) = o;
   };

@@ -75,7 +75,7 @@ __host__ __device__ inline int arith_mode(int spec_flags) { return ((spec_flags 
 //   (X + e*f) + t  -> fma(e, f, X) + t
 // at the projection of a voxel centre (voxel_centre, xform, project), every bilinear sample (depth, synthetic depth, colour /
 // feature taps, the low-res feature map incl. its source-index computation), the TSDF update's numerator and the appearance
-// blend's numerator -- in the oracle (fmaf) and here (v_fma_f32 / v_pk_fma_f32), same tree.  FMA is a template parameter like DIV:
+// blend's numerator -- in the oracle (fmaf) and here (v_fma_f32), same tree.  FMA is a template parameter like DIV:
 // the default kernels are not touched by it.
 template <int FMA>
 __device__ __forceinline__ float madd(float a, float b, float c) {
@@ -84,6 +84,13 @@ __device__ __forceinline__ float madd(float a, float b, float c) {
   else
     return a * b + c;
 }
+// float32 -> half of a computed value, rounded to float32 before it is rounded to half: without the barrier the compiler folds the
+// conversion into the last multiplication or addition (v_fma_mixlo_f16, one rounding instead of two; bits differ from the oracle's).
+__device__ __forceinline__ _Float16 half_of(float x) {
+  asm("" : "+v"(x));
+  return (_Float16)x;
+}
+
 // ---- scalar-register cap -------------------------------------------------------------------------------------------------------
 // The CU admits floor(800 / (ceil(sgpr / 16) * 16 + 16)) waves per SIMD (MI355X_MICROARCH.md, "Residency"): the per-voxel kernels'
 // natural 101-106 scalar registers mean SIX 256-thread workgroups per CU whatever the compiler's occupancy line says (7), and the

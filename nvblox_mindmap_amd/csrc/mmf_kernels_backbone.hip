@@ -126,7 +126,9 @@ __global__ __launch_bounds__(256, 2) void k_attn_split64(const float* __restrict
     const float4 a = p[0], c = p[1];
     // (log2 e rides in the scale: the exponentials below are bare v_exp_f32; one more rounding of q at 2^-24)
     const float sc = scale * 1.44269504088896340736f;
-    const float x[8] = {a.x * sc, a.y * sc, a.z * sc, a.w * sc, c.x * sc, c.y * sc, c.z * sc, c.w * sc};
+    float x[8] = {a.x * sc, a.y * sc, a.z * sc, a.w * sc, c.x * sc, c.y * sc, c.z * sc, c.w * sc};
+#pragma unroll
+    for (int t = 0; t < 8; ++t) asm volatile("" : "+v"(x[t]));  // (one value for the hi and the lo part: see k_split_act3_src)
     split8(x, qh[kk], ql[kk]);
   }
 

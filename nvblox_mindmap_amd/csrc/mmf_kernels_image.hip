@@ -378,7 +378,7 @@ __global__ __launch_bounds__(256) void k_upsample_features(const float* __restri
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const float val = madd2<FMA>(ly0, madd2<FMA>(lx0, a00.v[k], lx1, a01.v[k]), ly1, madd2<FMA>(lx0, a10.v[k], lx1, a11.v[k]));
-      o[k] = (_Float16)val;
+      o[k] = half_of(val);
     }
     *reinterpret_cast<half8*>(orow + (size_t)xf * Cpad) = o;
   }
