@@ -575,6 +575,54 @@ int mmf_adaln_modulate(const float* x_dev, const float* scale_shift_dev, float* 
 int mmf_attention_small(const float* q_dev, const float* k_dev, long long k_row_stride, const float* v_dev, long long v_row_stride,
                         const uint8_t* key_padding_dev, float* out_dev, int B, int Lq, int Lk, int heads, int head_dim, void* stream);
 
+/* ---- paged context memory ------------------------------------------------------------------------------------------------------
+ * Keys and values of growing contexts (a map that is explored over time, several robots with contexts of unlike length) in pages of
+ * page_size tokens, without padding; the policy's cross-attention reads them (mindmap/diffuser_actor/diffusion_head.py attends to one
+ * observation's context, projected anew each time).
+ *   keys    [num_pages, kv_heads, page_size, W]    a token's channels side by side
+ *   values  [num_pages, kv_heads, W, page_size]    a channel's tokens side by side
+ *   key_min, key_max [num_pages, kv_heads, W]      smallest / largest stored key of the page, channel by channel
+ *   table   [B, slots] int32   page of a context's tokens slot * page_size ..; an entry outside [0, num_pages) holds nothing: tokens that
+ *                              fall on it are not stored, and not attended to.  A page may stand in several contexts' tables (a shared
+ *                              beginning) as long as one call's tokens go to it from one context only.
+ *   lengths [B] int32          tokens a context holds; clamped to [0, slots * page_size]
+ * W = mmf_paged_width(head_dim): head_dim rounded up to 16, 32, 64, 96, 128 or 256; the channels behind head_dim are zero (allocate them
+ * so; nothing writes them).  page_size 16, 32, 64, 128 or 256.  Pools aligned to 16 bytes.  All sizes that depend on the device data
+ * (lengths, offsets, tables) are read on the device: a captured graph replays with new ones. */
+#define MMF_TYPE_F32 0
+#define MMF_TYPE_F16 1
+#define MMF_TYPE_BF16 2
+int mmf_paged_width(int head_dim);
+/* Rows offsets[b] .. offsets[b + 1] - 1 of k and v ([tokens, kv_heads * head_dim], row strides in elements, last dimension contiguous;
+ * the pages' type or float32) become tokens starts[b], starts[b] + 1, ... of context b; offsets [B + 1] int32 ascending, rows behind
+ * offsets[B] are not read; tokens beyond the table are not stored.  rotary_dim != 0: the keys' channel pairs (2 i, 2 i + 1) are rotated
+ * on the way by positions [tokens, axes] (float32): the first rotary_dim channels of every head, or of the whole row if rotary_dim ==
+ * kv_heads * head_dim; axis a has the channels [a, a + 1) * rotary_dim / axes, pair j of it turns by position_a * rotary_base^(-2 j axes /
+ * rotary_dim) -- with axes = 3 and the whole row the policy's code (mindmap/diffuser_actor/position_encodings.py).  Keys are rounded once
+ * to the pages' type; a page's key_min / key_max begin anew with the token in its first slot. */
+int mmf_paged_append(const void* k_dev, int64_t k_row_stride, const void* v_dev, int64_t v_row_stride, int in_type, int64_t tokens,
+                     const float* positions_dev, int axes, int rotary_dim, double rotary_base, const int32_t* offsets_dev,
+                     const int32_t* starts_dev, const int32_t* table_dev, int B, int slots, int page_size, int kv_heads, int head_dim,
+                     int num_pages, int type, void* keys_dev, void* values_dev, void* key_min_dev, void* key_max_dev, void* stream);
+/* out = softmax(scale q k^T) v of T query tokens per context over all its tokens: q, out [B, T, kv_heads * group * head_dim] of the pages'
+ * type; query head h reads key-value head h / group.  selected != null ([B, T, kv_heads, count] int32, table slots): over the tokens of
+ * these slots only (each at most once; an entry outside [0, slots) holds nothing).  No token: zeros.  Statistics and sums in 32 bits.
+ * The keys of a context are split over workgroups and joined by a second launch; workspace: mmf_paged_attention_workspace_bytes(...,
+ * capacity = (selected ? count : slots) * page_size, selected != 0) bytes, free again when the work is done. */
+int64_t mmf_paged_attention_workspace_bytes(int B, int T, int kv_heads, int group, int head_dim, int64_t capacity, int selected);
+int mmf_paged_attention(const void* q_dev, const void* keys_dev, const void* values_dev, int type, const int32_t* table_dev,
+                        const int32_t* lengths_dev, const int32_t* selected_dev, int count, int B, int T, int kv_heads, int group, int head_dim,
+                        int slots, int num_pages, int page_size, float scale, void* out_dev, void* workspace_dev, int64_t workspace_bytes,
+                        void* stream);
+/* The `count` table slots of every query token and key-value head with the highest scores, ascending, filled up with -1: selected
+ * [B, T, kv_heads, count].  A page's score is sum_c max(q_c, 0) key_max_c + min(q_c, 0) key_min_c -- no key of the page has a larger
+ * product with q --, the largest over the `group` query heads; in 64 bits, the lower slot first among equals.  A page whose score is not
+ * a number comes first.  workspace: mmf_paged_select_workspace_bytes bytes. */
+int64_t mmf_paged_select_workspace_bytes(int B, int T, int kv_heads, int slots);
+int mmf_paged_select(const void* q_dev, const void* key_min_dev, const void* key_max_dev, int type, const int32_t* table_dev,
+                     const int32_t* lengths_dev, int B, int T, int kv_heads, int group, int head_dim, int slots, int num_pages, int page_size,
+                     int count, int32_t* selected_dev, void* workspace_dev, int64_t workspace_bytes, void* stream);
+
 /* ---- diagnostics / measurement --------------------------------------------------------------- */
 /* Last sphere-traced synthetic depth image of the mapper: dims, then copy to out [Hs,Ws] f32. */
 int mmf_get_synthetic_depth_dims(mmf_handle h, int mapper_id, int* Hs, int* Ws);

@@ -207,6 +207,13 @@ SIGNATURES = {
     "mmf_attn_out_block": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _F, _VP, C.c_longlong, _I, _VP]),
     "mmf_ddpm_step": (_I, [_VP, _VP, C.c_longlong, _VP, _VP, C.c_longlong, _I, _I, _VP, _VP, _VP]),
     "mmf_attention_small": (_I, [_VP, _VP, C.c_longlong, _VP, C.c_longlong, _VP, _VP, _I, _I, _I, _I, _I, _VP]),
+    "mmf_paged_width": (_I, [_I]),
+    "mmf_paged_append": (_I, [_VP, C.c_int64, _VP, C.c_int64, _I, C.c_int64, _VP, _I, _I, C.c_double, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _VP,
+                              _VP, _VP, _VP, _VP]),
+    "mmf_paged_attention_workspace_bytes": (C.c_int64, [_I, _I, _I, _I, _I, C.c_int64, _I]),
+    "mmf_paged_attention": (_I, [_VP, _VP, _VP, _I, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _VP, _VP, C.c_int64, _VP]),
+    "mmf_paged_select_workspace_bytes": (C.c_int64, [_I, _I, _I, _I]),
+    "mmf_paged_select": (_I, [_VP, _VP, _VP, _I, _VP, _VP, _I, _I, _I, _I, _I, _I, _I, _I, _I, _VP, _VP, C.c_int64, _VP]),
     "mmf_farthest_point_sampling": (_I, [_VP, _I, _I, _I, _I, _I, _VP, _VP]),
     "mmf_fps_workspace_bytes": (C.c_int64, [_I, _I, _I]),
     "mmf_farthest_point_sampling_ws": (_I, [_VP, _I, _I, _I, _I, _I, _VP, _VP, C.c_int64, _VP]),

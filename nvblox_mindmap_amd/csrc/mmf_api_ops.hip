@@ -572,4 +572,84 @@ int mmf_attention_small(const float* q, const float* k, long long k_row_stride, 
   return check_launch();
 }
 
+int mmf_paged_width(int head_dim) { return paged_width(head_dim); }
+
+namespace {
+// what the three paged entry points share; 0, or a message
+const char* paged_shape_error(int type, int B, int slots, int page_size, int H, int head_dim, int num_pages) {
+  if (type < MMF_TYPE_F32 || type > MMF_TYPE_BF16) return "unknown element type";
+  if (B <= 0 || slots <= 0 || H <= 0 || num_pages <= 0) return "positive sizes";
+  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1))) return "page_size is 16, 32, 64, 128 or 256";
+  if (paged_width(head_dim) == 0) return "1 <= head_dim <= 256";
+  if ((int64_t)slots * page_size > 0x7fffff00LL) return "slots * page_size passes 31 bits";
+  return nullptr;
+}
+int page_shift(int page_size) { return __builtin_ctz((unsigned)page_size); }
+int paged_fail(const char* name, const char* why) { return fail(MMF_ERR_INVALID_ARG, std::string(name) + ": " + why); }
+}  // namespace
+
+int mmf_paged_append(const void* k, int64_t k_row_stride, const void* v, int64_t v_row_stride, int in_type, int64_t tokens, const float* positions,
+                     int axes, int rotary_dim, double rotary_base, const int32_t* offsets, const int32_t* starts, const int32_t* table, int B,
+                     int slots, int page_size, int kv_heads, int head_dim, int num_pages, int type, void* keys, void* values, void* key_min,
+                     void* key_max, void* stream) {
+  const char* name = "mmf_paged_append";
+  if (const char* e = paged_shape_error(type, B, slots, page_size, kv_heads, head_dim, num_pages)) return paged_fail(name, e);
+  if (tokens < 0 || tokens > 0x7fffffffLL) return paged_fail(name, "0 <= tokens < 2^31");
+  if (in_type != type && in_type != MMF_TYPE_F32) return paged_fail(name, "k and v are of the pages' type or float32");
+  if (!offsets || !starts || !table || !keys || !values || !key_min || !key_max) return paged_fail(name, "null pointer");
+  const int64_t row = (int64_t)kv_heads * head_dim;
+  if (row > 0x7fffffffLL) return paged_fail(name, "kv_heads * head_dim passes 31 bits");
+  if (rotary_dim) {
+    if (!positions || axes < 1 || axes > 4 || rotary_dim < 0 || rotary_dim % (2 * axes) || (rotary_dim > head_dim && rotary_dim != row) || !(rotary_base > 0))
+      return paged_fail(name, "rotary_dim is a multiple of 2 * axes, at most head_dim or kv_heads * head_dim, with positions of 1 to 4 axes");
+  }
+  if (tokens == 0) return MMF_OK;
+  if (!k || !v || k_row_stride < 0 || v_row_stride < 0) return paged_fail(name, "null or negatively strided k / v");
+  if (launch_paged_append(k, k_row_stride, v, v_row_stride, in_type, (int)tokens, positions, rotary_dim ? axes : 1, rotary_dim, rotary_base, offsets,
+                          starts, table, B, slots, page_shift(page_size), kv_heads, head_dim, num_pages, type, keys, values, key_min, key_max,
+                          (hipStream_t)stream) != 0)
+    return paged_fail(name, "types");
+  return check_launch();
+}
+
+int64_t mmf_paged_attention_workspace_bytes(int B, int T, int kv_heads, int group, int head_dim, int64_t capacity, int selected) {
+  if (B <= 0 || T <= 0 || kv_heads <= 0 || group <= 0 || paged_width(head_dim) == 0 || capacity < 0) return 0;
+  return 4 * (int64_t)paged_attention_workspace_floats(B, T, kv_heads, group, head_dim, capacity, selected != 0);
+}
+
+int mmf_paged_attention(const void* q, const void* keys, const void* values, int type, const int32_t* table, const int32_t* lengths,
+                        const int32_t* selected, int count, int B, int T, int kv_heads, int group, int head_dim, int slots, int num_pages,
+                        int page_size, float scale, void* out, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* name = "mmf_paged_attention";
+  if (const char* e = paged_shape_error(type, B, slots, page_size, kv_heads, head_dim, num_pages)) return paged_fail(name, e);
+  if (!q || !keys || !values || !table || !lengths || !out) return paged_fail(name, "null pointer");
+  if (T <= 0 || group <= 0 || (int64_t)T * group > (1 << 24) || (int64_t)kv_heads * group * head_dim > 0x7fffffffLL)
+    return paged_fail(name, "positive T and group");
+  if (selected && (count <= 0 || (int64_t)count * page_size > 0x7fffff00LL)) return paged_fail(name, "count > 0, count * page_size below 2^31");
+  const int64_t need = mmf_paged_attention_workspace_bytes(B, T, kv_heads, group, head_dim, (int64_t)(selected ? count : slots) * page_size, selected != nullptr);
+  if (workspace_bytes < need || (need > 0 && !workspace)) return paged_fail(name, "workspace smaller than mmf_paged_attention_workspace_bytes");
+  const int rc = launch_paged_attention(q, keys, values, type, table, lengths, selected, count, B, T, kv_heads, group, head_dim, slots, num_pages,
+                                        page_shift(page_size), scale, out, (float*)workspace, (hipStream_t)stream);
+  if (rc != 0) return paged_fail(name, "batch too large");
+  return check_launch();
+}
+
+int64_t mmf_paged_select_workspace_bytes(int B, int T, int kv_heads, int slots) {
+  return B > 0 && T > 0 && kv_heads > 0 && slots > 0 ? 8 * (int64_t)paged_select_workspace_doubles(B, T, kv_heads, slots) : 0;
+}
+
+int mmf_paged_select(const void* q, const void* key_min, const void* key_max, int type, const int32_t* table, const int32_t* lengths, int B, int T,
+                     int kv_heads, int group, int head_dim, int slots, int num_pages, int page_size, int count, int32_t* selected, void* workspace,
+                     int64_t workspace_bytes, void* stream) {
+  const char* name = "mmf_paged_select";
+  if (const char* e = paged_shape_error(type, B, slots, page_size, kv_heads, head_dim, num_pages)) return paged_fail(name, e);
+  if (!q || !key_min || !key_max || !table || !lengths || !selected || !workspace) return paged_fail(name, "null pointer");
+  if (T <= 0 || group <= 0 || count <= 0 || (int64_t)kv_heads * group * head_dim > 0x7fffffffLL) return paged_fail(name, "positive T, group and count");
+  if (workspace_bytes < mmf_paged_select_workspace_bytes(B, T, kv_heads, slots)) return paged_fail(name, "workspace smaller than mmf_paged_select_workspace_bytes");
+  if (launch_paged_select(q, key_min, key_max, type, table, lengths, B, T, kv_heads, group, head_dim, slots, num_pages, page_shift(page_size), count,
+                          (double*)workspace, selected, (hipStream_t)stream) != 0)
+    return paged_fail(name, "batch too large");
+  return check_launch();
+}
+
 }  // extern "C"

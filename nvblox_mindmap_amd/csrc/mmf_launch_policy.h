@@ -97,4 +97,18 @@ int launch_step_tail(const float* rot_seq, const float* pos_seq, long long seq_b
                      float* traj_out, const float* WeT, const float* be, const float* pos_table, const float* freq, float* tokens_out,
                      float* cos_out, float* sin_out, long long rot_batch_stride, hipStream_t s);
 
+
+// mmf_kernels_paged.hip (keys and values of growing contexts in pages: append, attention, page selection); types: 0 f32, 1 f16, 2 bf16
+int paged_width(int head_dim);
+int launch_paged_append(const void* k, long long k_stride, const void* v, long long v_stride, int in_type, int n_tokens, const float* positions,
+                        int axes, int rotary, double base, const int* offsets, const int* starts, const int* table, int B, int slots, int pshift,
+                        int H, int hd, int num_pages, int type, void* keys, void* values, void* kmin, void* kmax, hipStream_t s);
+long long paged_attention_workspace_floats(int B, int T, int H, int G, int hd, long long capacity, bool selected);
+int launch_paged_attention(const void* q, const void* keys, const void* values, int type, const int* table, const int* lengths, const int* selected,
+                           int count, int B, int T, int H, int G, int hd, int slots, int num_pages, int pshift, float scale, void* out, float* work,
+                           hipStream_t s);
+long long paged_select_workspace_doubles(int B, int T, int H, int slots);
+int launch_paged_select(const void* q, const void* kmin, const void* kmax, int type, const int* table, const int* lengths, int B, int T, int H, int G,
+                        int hd, int slots, int num_pages, int pshift, int count, double* work, int* out, hipStream_t s);
+
 }  // namespace mmf

@@ -1,0 +1,113 @@
+"""Refusals of the paged context operators, and the sizes they answer without a GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+from nvblox_mindmap_amd import _lib
+from nvblox_mindmap_amd.diffuser_actor import paged_context as P
+
+
+def pages(**change):
+    keys, values = torch.zeros(4, 2, 16, 32), torch.zeros(4, 2, 32, 16)
+    low, high = torch.zeros(4, 2, 32), torch.zeros(4, 2, 32)
+    d = dict(keys=keys, values=values, key_min=low, key_max=high, head_dim=20)
+    d.update(change)
+    return P.ContextPages(**d)
+
+
+def test_head_width_agrees_with_the_library():
+    L = _lib.lib()
+    for hd in range(1, 257):
+        assert P.head_width(hd) == L.mmf_paged_width(hd) >= hd
+    assert L.mmf_paged_width(0) == 0 and L.mmf_paged_width(257) == 0 and L.mmf_paged_width(-1) == 0
+    for hd in (0, 257):
+        with pytest.raises(ValueError):
+            P.head_width(hd)
+
+
+def test_no_cpu_fallback():
+    t = torch.zeros(1, 2, dtype=torch.int32)
+    one = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        P.context_attention(torch.zeros(1, 1, 40), pages(), t, one, 2)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        P.select_pages(torch.zeros(1, 1, 40), pages(), t, one, 2, 1)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        P.append_context(pages(), torch.zeros(1, 40), torch.zeros(1, 40), torch.zeros(2, dtype=torch.int32), one, t)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(keys=torch.zeros(4, 2, 24, 32)), "page_size"),
+    (dict(head_dim=33), "head_dim"),
+    (dict(head_dim=300), "head_dim"),
+    (dict(values=torch.zeros(4, 2, 16, 32)), "values"),
+    (dict(values=torch.zeros(4, 2, 32, 16, dtype=torch.float16)), "alike"),
+    (dict(keys=torch.zeros(4, 2, 16, 32, dtype=torch.float64)), "float32, float16 or bfloat16"),
+    (dict(keys=torch.zeros(4, 2, 32, 16).transpose(2, 3)), "contiguous"),
+    (dict(key_min=None), "key_min"),
+    (dict(key_max=torch.zeros(4, 2, 31)), "key_min"),
+    (dict(key_max=torch.zeros(4, 2, 32, dtype=torch.float16)), "key_min"),
+])
+def test_pages_are_checked(change, match):
+    with pytest.raises(ValueError, match=match):
+        P._check_pages(pages(**change), True)
+
+
+def test_allocation_is_checked():
+    for bad in (dict(page_size=48), dict(dtype=torch.int8), dict(head_dim=0), dict(num_pages=0), dict(kv_heads=0)):
+        args = dict(num_pages=2, kv_heads=2, head_dim=8, page_size=16, dtype=torch.float16, device="cpu")
+        args.update(bad)
+        with pytest.raises(ValueError):
+            P.allocate_pages(**args)
+    c = P.allocate_pages(3, 2, 15, 32, torch.bfloat16, "cpu")
+    assert c.keys.shape == (3, 2, 32, 16) and c.values.shape == (3, 2, 16, 32) and c.key_min.shape == (3, 2, 16) and c.page_size == 32
+
+
+def call_append(**change):
+    """The C entry with addresses that are never read: every case below is refused before a launch."""
+    fake = C.c_void_p(4096)
+    d = dict(k=fake, ks=40, v=fake, vs=40, in_type=0, tokens=3, positions=fake, axes=1, rotary=20, base=10000.0, offsets=fake, starts=fake, table=fake, B=1,
+             slots=2, page=16, heads=2, hd=20, num=4, type=0, keys=fake, values=fake, kmin=fake, kmax=fake, stream=None)
+    d.update(change)
+    return _lib.lib().mmf_paged_append(*d.values())
+
+
+@pytest.mark.parametrize("change", [dict(page=24), dict(page=8), dict(page=512), dict(hd=0), dict(hd=257), dict(type=3), dict(type=-1), dict(in_type=1),
+                                    dict(B=0), dict(slots=0), dict(slots=2 ** 28), dict(heads=0), dict(num=0), dict(tokens=-1), dict(tokens=2 ** 31),
+                                    dict(axes=0), dict(axes=5), dict(rotary=21), dict(rotary=22), dict(rotary=-2), dict(base=0.0), dict(positions=None), dict(k=None), dict(keys=None),
+                                    dict(kmin=None), dict(table=None), dict(ks=-1)])
+def test_append_refuses(change):
+    assert call_append(**change) != 0 and "mmf_paged_append" in _lib.last_error()
+
+
+def call_attention(**change):
+    fake = C.c_void_p(4096)
+    d = dict(q=fake, keys=fake, values=fake, type=0, table=fake, lengths=fake, selected=None, count=0, B=2, T=1, heads=2, group=1, hd=20, slots=100, num=4,
+             page=256, scale=1.0, out=fake, work=fake, bytes=1 << 40, stream=None)
+    d.update(change)
+    return _lib.lib().mmf_paged_attention(*d.values())
+
+
+@pytest.mark.parametrize("change", [dict(page=17), dict(hd=300), dict(type=7), dict(B=0), dict(T=0), dict(group=0), dict(slots=0), dict(slots=2 ** 24), dict(num=0),
+                                    dict(q=None), dict(lengths=None), dict(out=None), dict(bytes=0), dict(work=None),
+                                    dict(selected=C.c_void_p(4096), count=0), dict(T=2 ** 25)])
+def test_attention_refuses(change):
+    assert call_attention(**change) != 0 and "mmf_paged_attention" in _lib.last_error()
+
+
+@pytest.mark.parametrize("change", [dict(count=0), dict(T=0), dict(bytes=8), dict(work=None), dict(type=3), dict(page=0), dict(kmin=None), dict(group=0)])
+def test_selection_refuses(change):
+    fake = C.c_void_p(4096)
+    d = dict(q=fake, kmin=fake, kmax=fake, type=0, table=fake, lengths=fake, B=2, T=1, heads=2, group=1, hd=20, slots=100, num=4, page=16, count=3, out=fake,
+             work=fake, bytes=1 << 30, stream=None)
+    d.update(change)
+    assert _lib.lib().mmf_paged_select(*d.values()) != 0 and "mmf_paged_select" in _lib.last_error()
+
+
+def test_workspace_sizes():
+    L = _lib.lib()
+    assert L.mmf_paged_select_workspace_bytes(2, 3, 4, 5) == 8 * 120
+    assert L.mmf_paged_attention_workspace_bytes(1, 1, 1, 1, 16, 100, 0) == 0  # one split: no partial results
+    assert L.mmf_paged_attention_workspace_bytes(1, 1, 8, 4, 128, 1 << 20, 0) > 0
+    assert L.mmf_paged_attention_workspace_bytes(0, 1, 8, 4, 128, 1 << 20, 0) == 0
