@@ -671,128 +671,312 @@ struct SelectArgs {
   const void *q, *kmin, *kmax;
   const int *table, *lengths;
   int B, T, heads, H, G, hd, W, slots, num_pages, pshift, count;
-  double* scores;  // [B, T, H, slots]; -inf: the page is not there
+  int score_blocks, score_steps;  // workgroups of a (context, head), steps of each
+  double* scores;  // [B, T, H, slots]; -inf: the page is not there (entries behind the context's last page are not written)
   int* out;        // [B, T, H, count]
 };
 
+// One summary is read once: W / 8 lanes take 8 channels of a page each, 64 / that many pages side by side in a wave, two steps of them
+// at a time, all query rows over them.  The lanes' sums meet in a rotation within the 16-lane row, whose result is the same in
+// every lane.  (The 64-bit matrix instruction reaches 42 TFLOP/s here and pays for 16 rows whatever their number; four rows on
+// the vector unit cost less than the read.)
+template <int N>
+__device__ __forceinline__ double row_rotate(double x) {  // the value N lanes on in the row of 16
+  const long long u = __double_as_longlong(x);
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)u, 0x120 + N, 0xf, 0xf, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), 0x120 + N, 0xf, 0xf, false);
+  return __longlong_as_double(((long long)hi << 32) | (unsigned)lo);
+}
+// sum over groups of L neighbouring lanes, in every lane of the group
+template <int L>
+__device__ __forceinline__ double group_sum(double x) {
+  if constexpr (L >= 16) {
+    x += row_rotate<8>(x);
+    x += row_rotate<4>(x);
+    x += row_rotate<2>(x);
+    x += row_rotate<1>(x);
+    if constexpr (L == 32) x += __shfl_xor(x, 16);
+  } else {
+#pragma unroll
+    for (int d = L / 2; d > 0; d >>= 1) x += __shfl_xor(x, d);
+  }
+  return x;
+}
+
 template <class T>
-__global__ __launch_bounds__(256) void k_paged_score(SelectArgs a) {
-  const int page_slot = blockIdx.x * 256 + threadIdx.x;
-  if (page_slot >= a.slots) return;
-  const int h = blockIdx.y % a.H, b = blockIdx.y / a.H;
-  const int page = a.table[(long long)b * a.slots + page_slot];
-  const bool there = page >= 0 && page < a.num_pages && ((long long)page_slot << a.pshift) < a.lengths[b];
-  const T* mn = (const T*)a.kmin + ((long long)(there ? page : 0) * a.H + h) * a.W;
-  const T* mx = (const T*)a.kmax + ((long long)(there ? page : 0) * a.H + h) * a.W;
-  for (int t = 0; t < a.T; ++t) {
-    double best = -INFINITY;
-    if (there) {
-      for (int g = 0; g < a.G; ++g) {
-        const T* q = (const T*)a.q + (((long long)b * a.T + t) * a.heads + h * a.G + g) * a.hd;
-        double s = 0.0;
-        for (int c = 0; c < a.hd; ++c) {
-          const double x = (double)(float)q[c];
-          s = fma(x > 0.0 ? x : 0.0, (double)(float)mx[c], s);
-          s = fma(x < 0.0 ? x : 0.0, (double)(float)mn[c], s);
-        }
-        best = (s > best || s != s) ? s : best;
-        if (best != best) break;
-      }
-    }
-    a.scores[(((long long)b * a.T + t) * a.H + h) * a.slots + page_slot] = best;
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  constexpr int N = 16 / sizeof(T);
+#pragma unroll
+  for (int i = 0; i < 8 / N; ++i) {
+    const Pack<T, N> v = reinterpret_cast<const Pack<T, N>*>(p)[i];
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[N * i + j] = to_f(v.v[j]);
   }
 }
 
-// order-preserving key: larger score, larger key; -inf (not there) below all; NaN above all
+constexpr int kScoreRows = 4;  // query rows in registers at a time
+
+struct ScoreQuery {
+  double plus[kScoreRows][8], minus[kScoreRows][8];
+};
+template <class T>
+__device__ __forceinline__ void load_query(const SelectArgs& a, int b, int h, int r0, int rows, int c0, ScoreQuery& q) {
+#pragma unroll
+  for (int r = 0; r < kScoreRows; ++r) {
+    const int row = min(r0 + r, rows - 1);
+    const T* p = (const T*)a.q + (((long long)b * a.T + row / a.G) * a.heads + (long long)h * a.G + row % a.G) * a.hd;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const double x = c0 + j < a.hd ? (double)to_f(p[c0 + j]) : 0.0;
+      q.plus[r][j] = x > 0.0 ? x : (x != x ? x : 0.0);
+      q.minus[r][j] = x < 0.0 ? x : 0.0;
+    }
+  }
+}
+
+template <class T, int W>
+__global__ __launch_bounds__(256) void k_paged_score(SelectArgs a) {
+  constexpr int L = W == 96 ? 16 : W / 8, GP = 64 / L, STEP = 2 * GP;
+  const int unit = blockIdx.x / a.score_blocks, block = blockIdx.x % a.score_blocks;
+  const int h = unit % a.H, b = unit / a.H;
+  const int P = 1 << a.pshift;
+  const int np = (int)min((long long)a.slots, ((long long)max(a.lengths[b], 0) + P - 1) >> a.pshift);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c0 = (lane % L) * 8, gp = lane / L;
+  const int per_block = 4 * STEP * a.score_steps;
+  if (block * per_block >= np) return;
+  const int rows = a.T * a.G;
+  ScoreQuery q;
+  load_query<T>(a, b, h, 0, rows, c0, q);
+  for (int step = 0; step < a.score_steps; ++step) {
+    const int first = block * per_block + (step * 4 + wave) * STEP;
+    if (first >= np) break;
+    double mx[2][8], mn[2][8];
+    bool there[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int slot = first + i * GP + gp;
+      const int page = slot < np ? a.table[(long long)b * a.slots + slot] : -1;
+      there[i] = page >= 0 && page < a.num_pages;
+      float x[8];
+      const long long at = ((long long)(there[i] ? page : 0) * a.H + h) * W + c0;
+      if (W != 96 || c0 < W) load8((const T*)a.kmax + at, x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mx[i][j] = W != 96 || c0 < W ? (double)x[j] : 0.0;
+      if (W != 96 || c0 < W) load8((const T*)a.kmin + at, x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mn[i][j] = W != 96 || c0 < W ? (double)x[j] : 0.0;
+    }
+    double best[2] = {-INFINITY, -INFINITY};
+    for (int r0 = 0; r0 < rows; r0 += kScoreRows) {
+      if (rows > kScoreRows) load_query<T>(a, b, h, r0, rows, c0, q);
+#pragma unroll
+      for (int r = 0; r < kScoreRows; ++r) {
+        if (r0 + r >= rows) break;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          double s = 0.0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            s = fma(q.plus[r][j], mx[i][j], s);
+            s = fma(q.minus[r][j], mn[i][j], s);
+          }
+          s = group_sum<L>(s);
+          best[i] = (s > best[i] || s != s) ? s : best[i];
+        }
+        const int row = r0 + r;
+        if (row % a.G == a.G - 1) {
+          const int t = row / a.G;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int slot = first + i * GP + gp;
+            if (slot < np && lane % L == 0) a.scores[(((long long)b * a.T + t) * a.H + h) * a.slots + slot] = there[i] ? best[i] : -INFINITY;
+            best[i] = -INFINITY;
+          }
+        }
+      }
+    }
+  }
+}
+
+// order-preserving key: larger score, larger key; NaN above all; -inf (not there) at kNotThere, below all others
 __device__ __forceinline__ unsigned long long score_key(double s) {
   if (s != s) return ~0ull;
-  unsigned long long u = __double_as_longlong(s);
+  unsigned long long u = __double_as_longlong(s + 0.0);  // (-0 and 0 are equal)
   return (u >> 63) ? ~u : u | 0x8000000000000000ull;
 }
 constexpr unsigned long long kNotThere = 0x000fffffffffffffull;  // score_key(-inf)
 
-// The count best of a row, lowest slots first among equals: the threshold by radix selection (8 bits a pass), then one ordered pass that
-// writes the chosen slots in ascending order.
+// The count best of a row, the lowest slots first among equals, written in ascending order.  A threshold bucket is found by histogram
+// over [smallest, largest] key of the candidates: first over the scores themselves (2048 equal steps: scores spread over them whatever
+// their scale), then, in the bucket that holds the border, over the keys as integers, each time from their highest differing bit: 11 bits
+// a pass, so it ends.  Then one ordered pass writes what lies above the bucket, and of the last bucket's equals the first `need`.
+constexpr int kBuckets = 2048;
 __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
-  __shared__ int s_hist[256];
-  __shared__ int s_bin, s_need, s_left;
+  __shared__ int s_hist[kBuckets];
+  __shared__ unsigned long long s_lo[16], s_hi[16];
+  __shared__ int s_sum[16], s_bin, s_above;
   __shared__ int s_wave[2][16];
-  __shared__ int s_base[2];
   const long long row = blockIdx.x;
+  const int b = (int)(row / ((long long)a.T * a.H));
   const double* __restrict__ sc = a.scores + row * a.slots;
   int* __restrict__ out = a.out + row * a.count;
+  const int P = 1 << a.pshift;
+  const int np = (int)min((long long)a.slots, ((long long)max(a.lengths[b], 0) + P - 1) >> a.pshift);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  unsigned long long prefix = 0, mask = 0;
+  constexpr int R = 4;  // scores that a thread keeps (rows of up to 4096 pages are read once)
+  double mine[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) mine[i] = tid + 1024 * i < np ? sc[tid + 1024 * i] : -INFINITY;
+  auto score = [&](int i) { return i < R ? (i == 0 ? mine[0] : i == 1 ? mine[1] : i == 2 ? mine[2] : mine[3]) : sc[tid + 1024 * i]; };
+  const int mine_n = np > tid ? (np - tid + 1023) / 1024 : 0;
+
+  // candidates: keys in [lo, hi]; everything above hi is taken
+  unsigned long long lo = kNotThere + 1, hi = ~0ull;
   int need = a.count;
-  for (int shift = 56; shift >= 0; shift -= 8) {
-    if (tid < 256) s_hist[tid] = 0;
+  bool all = false, exact = false;
+  for (int pass = 0;; ++pass) {
+    unsigned long long mn = ~0ull, mx = 0;
+    int n = 0;
+    for (int i = 0; i < mine_n; ++i) {
+      const unsigned long long k = score_key(score(i));
+      if (k >= lo && k <= hi) {
+        mn = min(mn, k);
+        mx = max(mx, k);
+        ++n;
+      }
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      mn = min(mn, (unsigned long long)__shfl_xor((long long)mn, d));
+      mx = max(mx, (unsigned long long)__shfl_xor((long long)mx, d));
+      n += __shfl_xor(n, d);
+    }
+    if (lane == 0) {
+      s_lo[wave] = mn;
+      s_hi[wave] = mx;
+      s_sum[wave] = n;
+    }
+    for (int i = tid; i < kBuckets; i += 1024) s_hist[i] = 0;
     __syncthreads();
-    for (int i = tid; i < a.slots; i += 1024) {
-      const unsigned long long k = score_key(sc[i]);
-      if (k > kNotThere && (k & mask) == prefix) atomicAdd(&s_hist[(int)(k >> shift) & 255], 1);
+    n = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      mn = min(mn, s_lo[w]);
+      mx = max(mx, s_hi[w]);
+      n += s_sum[w];
+    }
+    if (n <= need) {  // all candidates
+      all = true;
+      if (n > 0) lo = mn;
+      break;
+    }
+    lo = mn;
+    hi = mx;
+    if (mn == mx) {  // equals: the first `need` of them
+      exact = true;
+      break;
+    }
+    const unsigned long long kInfKey = 0xfff0000000000000ull, kLowKey = kNotThere + 1;
+    const bool linear = pass == 0 && mx < kInfKey && mn >= kLowKey;  // (finite scores)
+    const double base = linear ? __longlong_as_double((mn >> 63) ? (long long)(mn & 0x7fffffffffffffffull) : (long long)~mn) : 0.0;
+    const double top = linear ? __longlong_as_double((mx >> 63) ? (long long)(mx & 0x7fffffffffffffffull) : (long long)~mx) : 0.0;
+    const double inv = linear ? (double)(kBuckets - 1) / (top - base) : 0.0;
+    const int shift = max(0, 64 - __clzll((long long)(mx - mn)) - 11);
+    // (a step that is no number, or infinite: all in one bucket, and the next pass goes by the integers)
+    auto bucket = [&](double s, unsigned long long k) { return linear ? min(max((int)((s - base) * inv), 0), kBuckets - 1) : (int)((k - mn) >> shift); };
+    for (int i = 0; i < mine_n; ++i) {
+      const double s = score(i);
+      const unsigned long long k = score_key(s);
+      if (k >= lo && k <= hi) atomicAdd(&s_hist[bucket(s, k)], 1);
     }
     __syncthreads();
-    if (tid == 0) {
-      int n = 0, bin = 255;
-      for (; bin >= 0; --bin) {
-        if (n + s_hist[bin] >= need) break;
-        n += s_hist[bin];
-      }
-      s_bin = bin;
-      s_need = need - n;
-      s_left = bin >= 0 ? s_hist[bin] : 0;
+    // the bucket that holds the border: counts from the top, two buckets a thread
+    const int b1 = kBuckets - 1 - 2 * tid, h1 = s_hist[b1], h0 = s_hist[b1 - 1];
+    int upto = h1 + h0;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(upto, d);
+      if (lane >= d) upto += o;
+    }
+    if (lane == 63) s_sum[wave] = upto;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) upto += s_sum[w];
+    const int before = upto - h1 - h0;
+    if (before < need && upto >= need) {
+      s_bin = before + h1 >= need ? b1 : b1 - 1;
+      s_above = before + h1 >= need ? before : before + h1;
     }
     __syncthreads();
     const int bin = s_bin;
-    if (bin < 0) break;  // fewer pages there than are wanted: all of them (in the first pass only)
-    need = s_need;
-    prefix |= (unsigned long long)bin << shift;
-    mask |= 255ull << shift;
-    if (s_left == need) break;  // all of this bin
-    __syncthreads();
-  }
-  const bool all = s_bin < 0;
-  const bool whole_bin = !all && s_left == need;
-  // keys above the threshold bin are chosen; of those in it the first `need`
-  if (tid < 2) s_base[tid] = 0;
-  __syncthreads();
-  for (int i0 = 0; i0 < a.slots; i0 += 1024) {
-    const int i = i0 + tid;
-    bool sure = false, maybe = false;
-    if (i < a.slots) {
-      const unsigned long long k = score_key(sc[i]);
-      if (k > kNotThere) {
-        if (all) sure = true;
-        else if ((k & mask) > prefix) sure = true;
-        else if ((k & mask) == prefix) {
-          sure = whole_bin;
-          maybe = !whole_bin;
-        }
+    need -= s_above;
+    // the bucket's own smallest and largest key are the next candidates' (found by the next pass's reduction)
+    unsigned long long bl = ~0ull, bh = 0;
+    for (int i = 0; i < mine_n; ++i) {
+      const double s = score(i);
+      const unsigned long long k = score_key(s);
+      if (k >= lo && k <= hi && bucket(s, k) == bin) {
+        bl = min(bl, k);
+        bh = max(bh, k);
       }
     }
-    const unsigned long long below = (1ull << lane) - 1;
-    const unsigned long long bm = __ballot(maybe);
-    if (lane == 0) s_wave[0][wave] = __popcll(bm);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      bl = min(bl, (unsigned long long)__shfl_xor((long long)bl, d));
+      bh = max(bh, (unsigned long long)__shfl_xor((long long)bh, d));
+    }
     __syncthreads();
-    int mb = s_base[0];
-    for (int w = 0; w < wave; ++w) mb += s_wave[0][w];
-    const bool take = sure || (maybe && mb + __popcll(bm & below) < need);
-    const unsigned long long bt = __ballot(take);
-    if (lane == 0) s_wave[1][wave] = __popcll(bt);
+    if (lane == 0) {
+      s_lo[wave] = bl;
+      s_hi[wave] = bh;
+    }
     __syncthreads();
-    int at = s_base[1];
-    for (int w = 0; w < wave; ++w) at += s_wave[1][w];
-    at += __popcll(bt & below);
-    if (take && at < a.count) out[at] = i;
-    __syncthreads();
-    if (tid == 0)
-      for (int w = 0; w < 16; ++w) {
-        s_base[0] += s_wave[0][w];
-        s_base[1] += s_wave[1][w];
-      }
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      bl = min(bl, s_lo[w]);
+      bh = max(bh, s_hi[w]);
+    }
+    lo = bl;
+    hi = bh;
     __syncthreads();
   }
-  for (int i = s_base[1] + tid; i < a.count; i += 1024) out[i] = -1;
+  // above hi: taken; in [lo, hi]: all of them, or the first `need`
+  int base_m = 0, base_t = 0;
+  for (int i = 0; i * 1024 < np; ++i) {
+    const int slot = i * 1024 + tid;
+    bool sure = false, maybe = false;
+    if (slot < np) {
+      const unsigned long long k = score_key(score(i));
+      if (k > kNotThere) {
+        sure = k > hi || (all && k >= lo);
+        maybe = exact && k == lo;
+      }
+    }
+    const unsigned long long below = (1ull << lane) - 1, bm = __ballot(maybe), bs = __ballot(sure);
+    if (lane == 0) {
+      s_wave[0][wave] = __popcll(bm);
+      s_wave[1][wave] = __popcll(bs);
+    }
+    __syncthreads();
+    int m = base_m, t = base_t, bm_all = 0, bs_all = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) {
+        m += s_wave[0][w];
+        t += s_wave[1][w];
+      }
+      bm_all += s_wave[0][w];
+      bs_all += s_wave[1][w];
+    }
+    m += __popcll(bm & below);
+    t += __popcll(bs & below);
+    // (of the equals before this slot, those that were taken: the first `need`)
+    const int at = t + min(m, exact ? need : 0);
+    if ((sure || (maybe && m < need)) && at < a.count) out[at] = slot;
+    base_m += bm_all;
+    base_t += bs_all;
+    __syncthreads();
+  }
+  for (int i = base_t + min(base_m, exact ? need : 0) + tid; i < a.count; i += 1024) out[i] = -1;
 }
 
 template <class TI, class T, int VEC, int VT>
@@ -831,6 +1015,18 @@ int attention_typed(const AttArgs& a, int W, int RT, int blocks, hipStream_t s) 
     case 256: attention_go<T, 256, 1>(a, blocks, s); return 0;
   }
   return 1;
+}
+
+template <class T>
+void score_typed(const SelectArgs& a, int blocks, hipStream_t s) {
+  switch (a.W) {
+    case 16: k_paged_score<T, 16><<<blocks, 256, 0, s>>>(a); break;
+    case 32: k_paged_score<T, 32><<<blocks, 256, 0, s>>>(a); break;
+    case 64: k_paged_score<T, 64><<<blocks, 256, 0, s>>>(a); break;
+    case 96: k_paged_score<T, 96><<<blocks, 256, 0, s>>>(a); break;
+    case 128: k_paged_score<T, 128><<<blocks, 256, 0, s>>>(a); break;
+    default: k_paged_score<T, 256><<<blocks, 256, 0, s>>>(a); break;
+  }
 }
 
 // rows of a unit go 16 or 32 at a time (one or two row tiles share a pass over the keys); heads of 256 channels leave registers for 16
@@ -911,15 +1107,20 @@ long long paged_select_workspace_doubles(int B, int T, int H, int slots) { retur
 
 int launch_paged_select(const void* q, const void* kmin, const void* kmax, int type, const int* table, const int* lengths, int B, int T, int H, int G,
                         int hd, int slots, int num_pages, int pshift, int count, double* work, int* out, hipStream_t s) {
-  if ((long long)B * H > 65535 || (long long)B * T * H > 0x7fffffffLL) return 2;
+  if ((long long)B * T * H > 0x7fffffffLL || (long long)T * G > 0x7fffffffLL) return 2;
   SelectArgs a{};
   a.q = q, a.kmin = kmin, a.kmax = kmax, a.table = table, a.lengths = lengths;
   a.B = B, a.T = T, a.heads = H * G, a.H = H, a.G = G, a.hd = hd, a.W = paged_width(hd), a.slots = slots, a.num_pages = num_pages, a.pshift = pshift;
   a.count = count, a.scores = work, a.out = out;
-  const dim3 grid((slots + 255) / 256, B * H);
-  if (type == 0) k_paged_score<float><<<grid, 256, 0, s>>>(a);
-  else if (type == 1) k_paged_score<_Float16><<<grid, 256, 0, s>>>(a);
-  else k_paged_score<__bf16><<<grid, 256, 0, s>>>(a);
+  const int L = a.W == 96 ? 16 : a.W / 8, per_step = 4 * 2 * (64 / L);  // pages of a workgroup's step
+  const long long all_steps = (long long)B * H * ((slots + per_step - 1) / per_step);
+  a.score_steps = (int)std::min(16LL, std::max(1LL, all_steps / 2048));  // about 8 workgroups a CU, each with its query loaded once
+  a.score_blocks = (slots + per_step * a.score_steps - 1) / (per_step * a.score_steps);
+  if ((long long)B * H * a.score_blocks > 0x7fffffffLL) return 2;
+  const int blocks = B * H * a.score_blocks;
+  if (type == 0) score_typed<float>(a, blocks, s);
+  else if (type == 1) score_typed<_Float16>(a, blocks, s);
+  else score_typed<__bf16>(a, blocks, s);
   k_paged_select<<<B * T * H, 1024, 0, s>>>(a);
   return 0;
 }

@@ -61,12 +61,35 @@ def allocate_pages(num_pages: int, kv_heads: int, head_dim: int, page_size: int 
                         zeros(num_pages, kv_heads, w), head_dim)
 
 
+# ---- checks: one expression on the way to the kernel (a call's host time is a good part of a small call), the reason only where it fails ----
+def _pages_ok(c: ContextPages, summary: bool) -> bool:
+    k, v = c.keys, c.values
+    if k.dim() != 4:
+        return False
+    n, h, p, w = k.shape
+    dtype, index = k.dtype, k.get_device()
+    ok = (dtype in _TYPES and v.dtype is dtype and p in PAGE_SIZES and n > 0 and h > 0 and 1 <= c.head_dim <= 256 and w == _WIDTH_OF[c.head_dim]
+          and v.shape == (n, h, w, p) and k.is_contiguous() and v.is_contiguous() and v.get_device() == index
+          and not (k.data_ptr() | v.data_ptr()) & 15)
+    if ok and summary:
+        lo, hi = c.key_min, c.key_max
+        ok = (lo is not None and hi is not None and lo.shape == (n, h, w) and hi.shape == (n, h, w) and lo.dtype is dtype and hi.dtype is dtype
+              and lo.is_contiguous() and hi.is_contiguous() and lo.get_device() == index and hi.get_device() == index
+              and not (lo.data_ptr() | hi.data_ptr()) & 15)
+    return ok
+
+
+_WIDTH_OF = (0,) + tuple(next(w for w in WIDTHS if w >= d) for d in range(1, WIDTHS[-1] + 1))
+
+
 def _check(cond: bool, what: str) -> None:
     if not cond:
         raise ValueError(what)
 
 
 def _check_pages(c: ContextPages, summary: bool) -> None:
+    if _pages_ok(c, summary):
+        return
     k, v = c.keys, c.values
     _check(k.dim() == 4 and v.dim() == 4, "keys [pages, kv_heads, page_size, W] and values [pages, kv_heads, W, page_size]")
     n, h, p, w = k.shape
@@ -75,41 +98,49 @@ def _check_pages(c: ContextPages, summary: bool) -> None:
     _check(w == head_width(c.head_dim), f"head_dim {c.head_dim} has pages of {head_width(c.head_dim)} channels, not {w}")
     _check(v.shape == (n, h, w, p), f"values {tuple(v.shape)} do not go with keys {tuple(k.shape)}")
     _check(n > 0 and h > 0, "no pages")
-    _check(k.is_contiguous() and v.is_contiguous() and k.data_ptr() % 16 == 0 and v.data_ptr() % 16 == 0, "pages are contiguous and 16-byte aligned")
     _check(v.device == k.device, "pages on one device")
-    if summary:
-        for s in (c.key_min, c.key_max):
-            _check(s is not None, "pages without key_min / key_max")
-            _check(s.shape == (n, h, w) and s.dtype == k.dtype and s.device == k.device and s.is_contiguous() and s.data_ptr() % 16 == 0,
-                   "key_min / key_max [pages, kv_heads, W] of the pages' type, contiguous, 16-byte aligned")
+    _check(not summary or (c.key_min is not None and c.key_max is not None), "pages without key_min / key_max")
+    for s in (c.key_min, c.key_max) if summary else ():
+        _check(s.shape == (n, h, w) and s.dtype == k.dtype and s.device == k.device, "key_min / key_max [pages, kv_heads, W] of the pages' type, on their device")
+    raise ValueError("pages are contiguous and 16-byte aligned")
 
 
-def _check_int(t: torch.Tensor, dim: int, device, name: str) -> None:
-    _check(t.dtype == torch.int32 and t.dim() == dim and t.device == device and t.is_contiguous(), f"{name}: a contiguous int32 tensor of {dim} dimension(s) on {device}")
+def _ints_ok(t: torch.Tensor, dim: int, index: int) -> bool:
+    return t.dtype is torch.int32 and t.dim() == dim and t.get_device() == index and t.is_contiguous()
 
 
-def _check_inputs(device, *ts: Optional[torch.Tensor]) -> None:
-    if device.type != "cuda":
+def _check_ints(device, **ts: torch.Tensor) -> None:
+    for name, (t, dim) in ts.items():
+        _check(_ints_ok(t, dim, device.index), f"{name}: a contiguous int32 tensor of {dim} dimension(s) on {device}")
+
+
+def _check_device(index: int, *ts: Optional[torch.Tensor]) -> None:
+    if index < 0:
         raise RuntimeError("paged contexts live on an MI355X (no CPU fallback)")
+    grad = torch.is_grad_enabled()
     for t in ts:
         if t is not None:
-            _check(t.device == device, f"all tensors on {device}: got one on {t.device}")
-            if t.requires_grad and torch.is_grad_enabled():
+            if t.get_device() != index:
+                raise ValueError(f"all tensors on cuda:{index}: got one on {t.device}")
+            if grad and t.requires_grad:
                 raise RuntimeError("paged contexts have no backward pass: call them under torch.no_grad(), or detach the inputs")
 
 
-def _on(device):
-    """The device current while a call launches (torch's default where it is already)."""
-    return torch.cuda.device(device)
+def _launch(index: int, entry, what: str, *args) -> None:
+    """entry(*args, stream) on the current stream of device `index`, which is made current for the call where it is not."""
+    current = torch._C._cuda_getDevice()
+    if current == index:
+        rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc, what)
 
 
 @functools.lru_cache(maxsize=512)
 def _attention_bytes(B, T, H, G, hd, capacity, selected) -> int:
     return int(_lib.lib().mmf_paged_attention_workspace_bytes(B, T, H, G, hd, capacity, selected))
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
 def append_context(context: ContextPages, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, starts: torch.Tensor, table: torch.Tensor,
@@ -124,47 +155,57 @@ def append_context(context: ContextPages, k: torch.Tensor, v: torch.Tensor, offs
 
     A page gets tokens of one context in a call (two that append to one page in the same call leave it undefined); pages that are only
     read may be shared."""
-    device = context.keys.device
-    _check_inputs(device, k, v, positions)
+    keys, hd = context.keys, context.head_dim
+    index = keys.get_device()
+    _check_device(index, k, v, positions)
     _check_pages(context, True)
-    n_pages, h, p, _ = context.keys.shape
-    row = h * context.head_dim
-    _check(k.dim() == 2 and k.shape == v.shape and k.shape[1] == row, f"k and v [n, {row}]: got {tuple(k.shape)}, {tuple(v.shape)}")
-    _check(k.dtype == v.dtype and k.dtype in (context.keys.dtype, torch.float32), f"k and v are {context.keys.dtype} or float32, both alike: got {k.dtype}, {v.dtype}")
-    _check_int(table, 2, device, "table")
-    _check_int(starts, 1, device, "starts")
-    _check_int(offsets, 1, device, "offsets")
+    n_pages, h, p, _ = keys.shape
+    row, n = h * hd, k.shape[0]
+    if not (k.dim() == 2 and k.shape == v.shape and k.shape[1] == row):
+        raise ValueError(f"k and v [n, {row}]: got {tuple(k.shape)}, {tuple(v.shape)}")
+    if not (k.dtype is v.dtype and (k.dtype is keys.dtype or k.dtype is torch.float32)):
+        raise ValueError(f"k and v are {keys.dtype} or float32, both alike: got {k.dtype}, {v.dtype}")
+    if not (_ints_ok(table, 2, index) and _ints_ok(starts, 1, index) and _ints_ok(offsets, 1, index)):
+        _check_ints(keys.device, table=(table, 2), starts=(starts, 1), offsets=(offsets, 1))
     b, slots = table.shape
-    _check(starts.shape[0] == b and offsets.shape[0] == b + 1, f"{b} contexts have {b} starts and {b + 1} offsets")
-    axes, rotary = 1, 0
+    if not (starts.shape[0] == b and offsets.shape[0] == b + 1):
+        raise ValueError(f"{b} contexts have {b} starts and {b + 1} offsets")
+    axes, rotary, at = 1, 0, 0
     if positions is not None:
-        _check(positions.dim() == 2 and positions.shape[0] == k.shape[0] and 1 <= positions.shape[1] <= 4 and positions.dtype == torch.float32
-               and positions.is_contiguous(), f"positions [{k.shape[0]}, axes] float32, contiguous, 1 to 4 axes")
-        axes, rotary = positions.shape[1], row if rotary_dim is None else int(rotary_dim)
-        _check(rotary > 0 and rotary % (2 * axes) == 0 and (rotary <= context.head_dim or rotary == row),
-               f"rotary_dim {rotary}: a multiple of {2 * axes}, at most head_dim {context.head_dim} or the whole row {row}")
-        _check(rotary_base > 0, "rotary_base has to be positive")
-    else:
-        _check(rotary_dim is None, "rotary_dim without positions")
-    if k.shape[0] == 0 or b == 0 or slots == 0:
+        if not (positions.dim() == 2 and positions.shape[0] == n and 1 <= positions.shape[1] <= 4 and positions.dtype is torch.float32
+                and positions.is_contiguous()):
+            raise ValueError(f"positions [{n}, axes] float32, contiguous, 1 to 4 axes")
+        axes, rotary, at = positions.shape[1], row if rotary_dim is None else int(rotary_dim), positions.data_ptr()
+        if not (rotary > 0 and rotary % (2 * axes) == 0 and (rotary <= hd or rotary == row)):
+            raise ValueError(f"rotary_dim {rotary}: a multiple of {2 * axes}, at most head_dim {hd} or the whole row {row}")
+        if not rotary_base > 0:
+            raise ValueError("rotary_base has to be positive")
+    elif rotary_dim is not None:
+        raise ValueError("rotary_dim without positions")
+    if n == 0 or b == 0 or slots == 0:
         return
-    k, v = _rows(k), _rows(v)
-    with _on(device):
-        _lib.check(_lib.lib().mmf_paged_append(_lib.dptr(k), k.stride(0), _lib.dptr(v), v.stride(0), _TYPES[k.dtype], k.shape[0], _lib.dptr(positions), axes,
-                                               rotary, float(rotary_base), _lib.dptr(offsets), _lib.dptr(starts), _lib.dptr(table), b, slots, p, h,
-                                               context.head_dim, n_pages, _TYPES[context.keys.dtype], _lib.dptr(context.keys), _lib.dptr(context.values),
-                                               _lib.dptr(context.key_min), _lib.dptr(context.key_max), _lib.stream_ptr(device)), "mmf_paged_append")
+    if k.stride(1) != 1:
+        k = k.contiguous()
+    if v.stride(1) != 1:
+        v = v.contiguous()
+    _launch(index, _lib.lib().mmf_paged_append, "mmf_paged_append", k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), _TYPES[k.dtype], n, at, axes,
+            rotary, rotary_base, offsets.data_ptr(), starts.data_ptr(), table.data_ptr(), b, slots, p, h, hd, n_pages, _TYPES[keys.dtype], keys.data_ptr(),
+            context.values.data_ptr(), context.key_min.data_ptr(), context.key_max.data_ptr())
 
 
-def _check_query(q: torch.Tensor, context: ContextPages, table: torch.Tensor, lengths: torch.Tensor, heads: int):
-    device = context.keys.device
-    h = context.keys.shape[1]
-    _check(heads > 0 and heads % h == 0, f"heads {heads}: a multiple of the {h} key-value heads")
-    _check(q.dim() == 3 and q.shape[2] == heads * context.head_dim, f"q [contexts, tokens, {heads * context.head_dim}]: got {tuple(q.shape)}")
-    _check(q.dtype == context.keys.dtype, f"q is {q.dtype}, the pages are {context.keys.dtype}")
-    _check_int(table, 2, device, "table")
-    _check_int(lengths, 1, device, "lengths")
-    _check(table.shape[0] == q.shape[0] == lengths.shape[0], f"{q.shape[0]} contexts: table {tuple(table.shape)}, lengths {tuple(lengths.shape)}")
+def _check_query(q: torch.Tensor, context: ContextPages, table: torch.Tensor, lengths: torch.Tensor, heads: int, index: int) -> None:
+    keys = context.keys
+    h = keys.shape[1]
+    if not (heads > 0 and heads % h == 0):
+        raise ValueError(f"heads {heads}: a multiple of the {h} key-value heads")
+    if not (q.dim() == 3 and q.shape[2] == heads * context.head_dim):
+        raise ValueError(f"q [contexts, tokens, {heads * context.head_dim}]: got {tuple(q.shape)}")
+    if q.dtype is not keys.dtype:
+        raise ValueError(f"q is {q.dtype}, the pages are {keys.dtype}")
+    if not (_ints_ok(table, 2, index) and _ints_ok(lengths, 1, index)):
+        _check_ints(keys.device, table=(table, 2), lengths=(lengths, 1))
+    if not table.shape[0] == q.shape[0] == lengths.shape[0]:
+        raise ValueError(f"{q.shape[0]} contexts: table {tuple(table.shape)}, lengths {tuple(lengths.shape)}")
 
 
 def context_attention(q: torch.Tensor, context: ContextPages, table: torch.Tensor, lengths: torch.Tensor, heads: int,
@@ -173,29 +214,31 @@ def context_attention(q: torch.Tensor, context: ContextPages, table: torch.Tenso
     [contexts, T, heads * head_dim] of the pages' type, rotated by the caller (``fused_ops.rotary_apply``, ``q_block``); query head i reads
     key-value head i // (heads / kv_heads).  ``pages`` [contexts, T, kv_heads, count] int32 (``select_pages``): over the tokens of these
     table slots only; an entry outside the table holds nothing, none may stand twice.  Zeros where there is no token.  -> [contexts, T, heads * head_dim]."""
-    device = context.keys.device
-    _check_inputs(device, q, table, lengths)
+    keys, hd = context.keys, context.head_dim
+    index = keys.get_device()
+    _check_device(index, q)
     _check_pages(context, False)
-    _check_query(q, context, table, lengths, heads)
-    n_pages, h, p, _ = context.keys.shape
+    _check_query(q, context, table, lengths, heads, index)
+    n_pages, h, p, _ = keys.shape
     b, t, _ = q.shape
-    slots, count = table.shape[1], 0
+    slots, count, chosen = table.shape[1], 0, 0
     if pages is not None:
-        _check_int(pages, 4, device, "pages")
-        _check(pages.shape[:3] == (b, t, h), f"pages [{b}, {t}, {h}, count]: got {tuple(pages.shape)}")
-        count = pages.shape[3]
-    if q.numel() == 0 or slots == 0 or (pages is not None and count == 0):
-        return torch.zeros(q.shape, dtype=q.dtype, device=device)
-    q = q.contiguous()
+        if not _ints_ok(pages, 4, index):
+            _check_ints(keys.device, pages=(pages, 4))
+        count, chosen = pages.shape[3], pages.data_ptr()
+        if pages.shape != (b, t, h, count):
+            raise ValueError(f"pages [{b}, {t}, {h}, count]: got {tuple(pages.shape)}")
+    if b == 0 or t == 0 or slots == 0 or (pages is not None and count == 0):
+        return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    if not q.is_contiguous():
+        q = q.contiguous()
     out = torch.empty_like(q)
-    need = _attention_bytes(b, t, h, heads // h, context.head_dim, (slots if pages is None else count) * p, int(pages is not None))
+    need = _attention_bytes(b, t, h, heads // h, hd, (slots if pages is None else count) * p, int(pages is not None))
     # per call, from torch's caching allocator: safe inside a captured graph (its private pool) and across streams
-    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    with _on(device):
-        _lib.check(_lib.lib().mmf_paged_attention(_lib.dptr(q), _lib.dptr(context.keys), _lib.dptr(context.values), _TYPES[q.dtype], _lib.dptr(table),
-                                                  _lib.dptr(lengths), _lib.dptr(pages), count, b, t, h, heads // h, context.head_dim, slots, n_pages, p,
-                                                  context.head_dim ** -0.5 if scale is None else float(scale), _lib.dptr(out), _lib.dptr(work), need,
-                                                  _lib.stream_ptr(device)), "mmf_paged_attention")
+    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _launch(index, _lib.lib().mmf_paged_attention, "mmf_paged_attention", q.data_ptr(), keys.data_ptr(), context.values.data_ptr(), _TYPES[q.dtype],
+            table.data_ptr(), lengths.data_ptr(), chosen, count, b, t, h, heads // h, hd, slots, n_pages, p, hd ** -0.5 if scale is None else scale,
+            out.data_ptr(), work.data_ptr() if need else 0, need)
     return out
 
 
@@ -204,22 +247,23 @@ def select_pages(q: torch.Tensor, context: ContextPages, table: torch.Tensor, le
     [contexts, T, kv_heads, count] int32, ascending, filled up with -1 -- the ``pages`` of ``context_attention``.  A page's score is
     sum_c max(q_c, 0) key_max_c + min(q_c, 0) key_min_c, which no key of the page exceeds, the largest over the query heads that share the
     key-value head; taken in 64 bits, the lower slot first among equals."""
-    device = context.keys.device
-    _check_inputs(device, q, table, lengths)
+    keys, hd = context.keys, context.head_dim
+    index = keys.get_device()
+    _check_device(index, q)
     _check_pages(context, True)
-    _check_query(q, context, table, lengths, heads)
-    _check(count > 0, "count has to be positive")
-    n_pages, h, p, _ = context.keys.shape
+    _check_query(q, context, table, lengths, heads, index)
+    if not count > 0:
+        raise ValueError("count has to be positive")
+    n_pages, h, p, _ = keys.shape
     b, t, _ = q.shape
     slots = table.shape[1]
-    if q.numel() == 0 or slots == 0:
-        return torch.full((b, t, h, count), -1, dtype=torch.int32, device=device)
-    q = q.contiguous()
-    out = torch.empty((b, t, h, count), dtype=torch.int32, device=device)
+    if b == 0 or t == 0 or slots == 0:
+        return torch.full((b, t, h, count), -1, dtype=torch.int32, device=q.device)
+    if not q.is_contiguous():
+        q = q.contiguous()
+    out = torch.empty((b, t, h, count), dtype=torch.int32, device=q.device)
     need = 8 * b * t * h * slots
-    work = torch.empty(need, dtype=torch.uint8, device=device)
-    with _on(device):
-        _lib.check(_lib.lib().mmf_paged_select(_lib.dptr(q), _lib.dptr(context.key_min), _lib.dptr(context.key_max), _TYPES[q.dtype], _lib.dptr(table),
-                                               _lib.dptr(lengths), b, t, h, heads // h, context.head_dim, slots, n_pages, p, count, _lib.dptr(out),
-                                               _lib.dptr(work), need, _lib.stream_ptr(device)), "mmf_paged_select")
+    work = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _launch(index, _lib.lib().mmf_paged_select, "mmf_paged_select", q.data_ptr(), context.key_min.data_ptr(), context.key_max.data_ptr(), _TYPES[q.dtype],
+            table.data_ptr(), lengths.data_ptr(), b, t, h, heads // h, hd, slots, n_pages, p, count, out.data_ptr(), work.data_ptr(), need)
     return out
