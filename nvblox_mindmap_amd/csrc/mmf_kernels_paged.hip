@@ -13,6 +13,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <numeric>
 
 #include "mmf_device.h"
 #include "mmf_launch_policy.h"
@@ -28,6 +29,11 @@ typedef short s4v __attribute__((ext_vector_type(4)));
 
 template <class T, int N>
 struct alignas(sizeof(T) * N) Pack {
+  T v[N];
+};
+
+template <class T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) Loose {  // the same, aligned like one element
   T v[N];
 };
 
@@ -68,12 +74,14 @@ struct Segment {
   int b, slot, first, last, row;  // context, table slot, slots [first, last) of the page, row of slot `first`'s token
 };
 
-// The unit-th (context, page) pair that gets tokens: contexts in order, pages in order.
+// The unit-th (context, page) pair that gets tokens: contexts in order, pages in order.  One thread a context, a scan over the
+// workgroup.
 __device__ __forceinline__ bool find_segment(const AppendArgs& a, int unit, Segment& s) {
-  const int lane = threadIdx.x & 63, P = 1 << a.pshift;
+  __shared__ int s_total[4], s_seg[5];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, P = 1 << a.pshift;
   int before = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int b = b0 + lane;
+  for (int b0 = 0; b0 < a.B; b0 += 256) {
+    const int b = b0 + tid;
     int lo = 0, n = 0, st = 0, np = 0;
     if (b < a.B) {
       lo = min(max(a.offsets[b], 0), a.n_tokens);
@@ -91,166 +99,210 @@ __device__ __forceinline__ bool find_segment(const AppendArgs& a, int unit, Segm
       const int o = __shfl_up(upto, d);
       if (lane >= d) upto += o;
     }
-    const unsigned long long hit = __ballot(before + upto > unit);
-    if (hit) {
-      const int src = __ffsll(hit) - 1;
-      const int base = before + __shfl(upto, src) - __shfl(np, src);
-      const int st_ = __shfl(st, src), n_ = __shfl(n, src), lo_ = __shfl(lo, src);
-      s.b = b0 + src;
-      s.slot = (st_ >> a.pshift) + unit - base;
-      const int page_first = s.slot << a.pshift;
-      s.first = max(st_ - page_first, 0);
-      s.last = min(st_ + n_ - page_first, P);
-      s.row = lo_ + page_first + s.first - st_;
+    if (lane == 63) s_total[wave] = upto;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) upto += s_total[w];
+      all += s_total[w];
+    }
+    if (before + all > unit) {
+      if (before + upto > unit && before + upto - np <= unit) {
+        const int slot = (st >> a.pshift) + unit - (before + upto - np), page_first = slot << a.pshift, first = max(st - page_first, 0);
+        s_seg[0] = b;
+        s_seg[1] = slot;
+        s_seg[2] = first;
+        s_seg[3] = min(st + n - page_first, P);
+        s_seg[4] = lo + page_first + first - st;
+      }
+      __syncthreads();
+      s.b = s_seg[0], s.slot = s_seg[1], s.first = s_seg[2], s.last = s_seg[3], s.row = s_seg[4];
       return true;
     }
-    before += __shfl(upto, 63);
+    before += all;
+    __syncthreads();
   }
   return false;
 }
 
-// cos / sin of the angle of channel pair `within` / 2 at a position: position * base^(-2 j / span), taken in turns and reduced in 64
-// bits (a far position times a frequency loses its fraction in 32), then in 32 bits on [-1/2, 1/2] turns.
-__device__ __forceinline__ double turns_per_unit(int within, int span, double log2_base) {
-  const int j2 = (within % span) & ~1;
-  return exp2(-log2_base * (double)j2 / (double)span) * 0.15915494309189533576888;
-}
-__device__ __forceinline__ void turn(float position, double freq, float& c, float& s) {
-  const double t = (double)position * freq;
-  sincospif(2.0f * (float)(t - rint(t)), &s, &c);
-}
-
+// VEC > 1: VEC neighbouring channels of the row (of one head or of two), whose rotation pairs are the lane's own; VEC == 1: any layout,
+// the partner is read beside it.  The page is taken in blocks of tokens whose cos / sin fit into LDS: computed once for all
+// heads (of the row's own pairs where the code covers the whole row), which takes them out of the registers and off the 128-byte
+// lines that bound the kernel.
+constexpr int kAngles = 4096, kAppendRow = 1024;  // entries of the table; channels of a workgroup at most
 template <class TI, class T, int VEC, int VT>
 __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
+  __shared__ float2 s_angle[kAngles];               // [token of the block][pair]: cos, sin
+  __shared__ double s_turns[kAppendRow / 2];        // turns a unit of position, by pair
+  __shared__ float s_lo[kAppendRow], s_hi[kAppendRow];
   Segment seg;
   if (!find_segment(a, blockIdx.x, seg)) return;
   const int page = a.table[(long long)seg.b * a.slots + seg.slot];
   if (page < 0 || page >= a.num_pages) return;
+  const int tid = threadIdx.x;
   const int h0 = blockIdx.y * a.heads_per_wg, nh = min(a.heads_per_wg, a.H - h0);
-  const int chunks_per_head = a.hd / VEC, nchunks = nh * chunks_per_head;
-  const int g0 = seg.first / VT, ng = (seg.last - 1) / VT + 1 - g0;
-  int gw = 1;  // neighbouring lanes take neighbouring slot groups: 8 of them fill the value rows' cache lines
-  while (gw < 8 && gw < ng) gw <<= 1;
-  const int gl = threadIdx.x & (gw - 1);
+  const int c0 = h0 * a.hd, nchunks = nh * a.hd / VEC;
+  const bool whole_row = a.rotary > a.hd;
+  const int pairs = a.rotary ? (whole_row ? (nh * a.hd + 1 + (c0 & 1)) / 2 : a.rotary / 2) : 0;  // (a whole row's pairs may begin before h0's first channel)
+  const int pair0 = whole_row ? c0 / 2 : 0;
+  const int span = a.rotary ? a.rotary / a.axes : 2;
   const TI* __restrict__ kin = (const TI*)a.k;
   const TI* __restrict__ vin = (const TI*)a.v;
   const long long page_head = (long long)page * a.H;
-  for (int ch = threadIdx.x / gw; ch < nchunks; ch += 256 / gw) {
-    const int h = h0 + ch / chunks_per_head, d = (ch % chunks_per_head) * VEC;
-    const int c = h * a.hd + d;  // channel in the row
-    const int within = a.rotary > a.hd ? c : d;
-    const int span = a.rotary ? a.rotary / a.axes : 1;
-    T* __restrict__ kp = (T*)a.keys + ((page_head + h) << a.pshift) * a.W + d;
-    T* __restrict__ vp = (T*)a.values + (((page_head + h) * a.W + d) << a.pshift);
-    // VEC > 1: the pairs are the lane's own; VEC == 1: the partner is the neighbouring channel
-    constexpr int NPAIR = VEC > 1 ? VEC / 2 : 1;
-    double freq[NPAIR];
-    int axis[NPAIR];
+  for (int i = tid; i < pairs; i += 256) {
+    const int j = (2 * (pair0 + i)) % span;  // pair j / 2 of its axis: position * base^(-j / span) / 2 pi turns
+    s_turns[i] = exp2(-a.log2_base * (double)j / (double)span) * 0.15915494309189533576888;
+  }
+  const int block = pairs ? min(256, kAngles / pairs / VT * VT) : 256;  // tokens of a block
+  // what the page's summary held (it begins anew with its first slot), asked for early: the first access to a page of a large pool waits long
+  constexpr int OLD = kAppendRow / 256;
+  const bool merge = seg.first > 0;
+  float old_lo[OLD], old_hi[OLD];
+  if (merge) {
 #pragma unroll
-    for (int i = 0; i < NPAIR; ++i) {
-      const int w = within + 2 * i;
-      const bool on = w < a.rotary;
-      axis[i] = on ? w / span : -1;
-      freq[i] = on ? turns_per_unit(w, span, a.log2_base) : 0.0;
+    for (int j = 0; j < OLD; ++j) {
+      const int i = min(tid + 256 * j, nh * a.hd - 1);
+      const long long at = (page_head + h0 + i / a.hd) * a.W + i % a.hd;
+      old_lo[j] = to_f(((const T*)a.kmin)[at]);
+      old_hi[j] = to_f(((const T*)a.kmax)[at]);
     }
-    float lo[VEC], hi[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      lo[i] = INFINITY;
-      hi[i] = -INFINITY;
+  }
+  bool begun = false;
+  for (int first = seg.first / VT * VT; first < seg.last; first += block) {
+    const int lo_slot = max(first, seg.first), hi_slot = min(first + block, seg.last);
+    if (pairs) {
+      __syncthreads();
+      const int n = (hi_slot - lo_slot) * pairs;
+      for (int i = tid; i < n; i += 256) {
+        const int t = i / pairs, w = i - t * pairs, axis = 2 * (pair0 + w) / span;
+        const long long row = seg.row + (lo_slot + t - seg.first);
+        // taken in turns and reduced in 64 bits (a far position times a frequency loses its fraction in 32), then in 32 on [-1/2, 1/2]
+        const double turns = (double)a.positions[row * a.axes + axis] * s_turns[w];
+        float2 cs;
+        sincospif(2.0f * (float)(turns - rint(turns)), &cs.y, &cs.x);
+        s_angle[(lo_slot + t - first) * pairs + w] = cs;
+      }
+      __syncthreads();
     }
-    for (int g = gl; g < ng; g += gw) {
-      const int slot0 = (g0 + g) * VT;
-      T vt[VEC][VT];
+    const int ng = (hi_slot - first + VT - 1) / VT;
+    int gw = 1;  // neighbouring lanes take neighbouring slot groups: 8 of them fill the value rows' cache lines
+    while (gw < 8 && gw < ng) gw <<= 1;
+    const int gl = tid & (gw - 1);
+    for (int ch = tid / gw; ch < nchunks; ch += 256 / gw) {
+      const int c = c0 + ch * VEC;  // channel in the row
+      const int h = c / a.hd, d = c - h * a.hd;
+      const bool one_head = d + VEC <= a.hd;
+      float lo[VEC], hi[VEC];
 #pragma unroll
-      for (int t = 0; t < VT; ++t) {
-        const int slot = slot0 + t;
-        const bool in = slot >= seg.first && slot < seg.last;
-        if (!in) continue;
-        const long long row = seg.row + (slot - seg.first);
-        float x[VEC];
-        const TI* kr = kin + row * a.k_stride + c;
-        const TI* vr = vin + row * a.v_stride + c;
-        if constexpr (VEC > 1) {
-          const Pack<TI, VEC> kv = *reinterpret_cast<const Pack<TI, VEC>*>(kr);
-          const Pack<TI, VEC> vv = *reinterpret_cast<const Pack<TI, VEC>*>(vr);
+      for (int i = 0; i < VEC; ++i) {
+        lo[i] = INFINITY;
+        hi[i] = -INFINITY;
+      }
+      for (int g = gl; g < ng; g += gw) {
+        const int slot0 = first + g * VT;
+        const bool full = slot0 >= seg.first && slot0 + VT <= seg.last;
+        // all loads first (a slot outside the block's tokens reads the nearest inside: its values count twice in the summary, which is the same)
+        Pack<TI, VEC> kr[VT], vr[VT];
+#pragma unroll
+        for (int t = 0; t < VT; ++t) {
+          const long long row = (long long)seg.row + (min(max(slot0 + t, lo_slot), hi_slot - 1) - seg.first);
+          kr[t] = *reinterpret_cast<const Pack<TI, VEC>*>(kin + row * a.k_stride + c);
+          vr[t] = *reinterpret_cast<const Pack<TI, VEC>*>(vin + row * a.v_stride + c);
+        }
+#pragma unroll
+        for (int t = 0; t < VT; ++t) {
+          const int slot = min(max(slot0 + t, lo_slot), hi_slot - 1);
+          float x[VEC];
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) x[i] = to_f(kr[t].v[i]);
+          if (pairs) {
+            const float2* angle = s_angle + (slot - first) * pairs;
+            if constexpr (VEC > 1) {
+#pragma unroll
+              for (int i = 0; i < VEC / 2; ++i) {
+                const int w = whole_row ? c + 2 * i : one_head ? d + 2 * i : (c + 2 * i) % a.hd;
+                if (w < a.rotary) {
+                  const float2 cs = angle[w / 2 - pair0];
+                  const float e = x[2 * i], o = x[2 * i + 1];
+                  x[2 * i] = e * cs.x - o * cs.y;
+                  x[2 * i + 1] = o * cs.x + e * cs.y;
+                }
+              }
+            } else {
+              const int w = whole_row ? c : d;
+              if (w < a.rotary) {
+                const float2 cs = angle[w / 2 - pair0];
+                const long long row = (long long)seg.row + (slot - seg.first);
+                const float p = to_f(kin[row * a.k_stride + c + ((w & 1) ? -1 : 1)]);
+                x[0] = (w & 1) ? x[0] * cs.x + p * cs.y : x[0] * cs.x - p * cs.y;
+              }
+            }
+          }
+          Pack<T, VEC> out;
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
-            x[i] = to_f(kv.v[i]);
-            vt[i][t] = (T)to_f(vv.v[i]);
+            out.v[i] = stored<T>(x[i]);  // the one rounding of a key; the summary is of the stored value
+            const float y = to_f(out.v[i]);
+            lo[i] = smaller(lo[i], y);
+            hi[i] = larger(hi[i], y);
           }
-          if (a.rotary) {
+          if (full || slot == slot0 + t) {
+            T* kp = (T*)a.keys + ((page_head + h) << a.pshift) * a.W + (long long)slot * a.W + d;
+            if (one_head) {
+              *reinterpret_cast<Loose<T, VEC>*>(kp) = __builtin_bit_cast(Loose<T, VEC>, out);  // (16 bytes, aligned like the type)
+            } else {
 #pragma unroll
-            for (int i = 0; i < NPAIR; ++i)
-              if (axis[i] >= 0) {
-                float cs, sn;
-                turn(a.positions[row * a.axes + axis[i]], freq[i], cs, sn);
-                const float e = x[2 * i], o = x[2 * i + 1];
-                x[2 * i] = e * cs - o * sn;
-                x[2 * i + 1] = o * cs + e * sn;
+              for (int i = 0; i < VEC; ++i) {
+                const int hh = (c + i) / a.hd, dd = (c + i) % a.hd;
+                ((T*)a.keys)[((page_head + hh) << a.pshift) * a.W + (long long)slot * a.W + dd] = out.v[i];
               }
-          }
-        } else {
-          x[0] = to_f(kr[0]);
-          vt[0][t] = (T)to_f(vr[0]);
-          if (axis[0] >= 0) {
-            float cs, sn;
-            turn(a.positions[row * a.axes + axis[0]], freq[0], cs, sn);
-            const bool odd = within & 1;
-            const float p = to_f(kr[odd ? -1 : 1]);
-            x[0] = odd ? x[0] * cs + p * sn : x[0] * cs - p * sn;
+            }
           }
         }
-        Pack<T, VEC> out;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          out.v[i] = stored<T>(x[i]);  // the one rounding of a key; the summary is of the stored value
-          const float y = to_f(out.v[i]);
-          lo[i] = smaller(lo[i], y);
-          hi[i] = larger(hi[i], y);
-        }
-        if constexpr (VEC > 1)
-          *reinterpret_cast<Pack<T, VEC>*>(kp + (long long)slot * a.W) = out;
-        else
-          kp[(long long)slot * a.W] = out.v[0];
-      }
-      if (slot0 >= seg.first && slot0 + VT <= seg.last) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
+          const int hh = one_head ? h : (c + i) / a.hd, dd = one_head ? d + i : (c + i) % a.hd;
+          T* vp = (T*)a.values + (((page_head + hh) * a.W + dd) << a.pshift) + slot0;
           Pack<T, VT> out;
 #pragma unroll
-          for (int t = 0; t < VT; ++t) out.v[t] = vt[i][t];
-          *reinterpret_cast<Pack<T, VT>*>(vp + ((long long)i << a.pshift) + slot0) = out;
-        }
-      } else {
+          for (int t = 0; t < VT; ++t) out.v[t] = (T)to_f(vr[t].v[i]);
+          if (full) {
+            *reinterpret_cast<Pack<T, VT>*>(vp) = out;
+          } else {
 #pragma unroll
-        for (int t = 0; t < VT; ++t)
-          if (slot0 + t >= seg.first && slot0 + t < seg.last) {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) vp[((long long)i << a.pshift) + slot0 + t] = vt[i][t];
+            for (int t = 0; t < VT; ++t)
+              if (slot0 + t >= lo_slot && slot0 + t < hi_slot) vp[t] = out.v[t];
           }
+        }
       }
-    }
-    // over the gw lanes of this chunk, then with what the page held before (a page's summary begins with its first slot)
-    T* __restrict__ mn = (T*)a.kmin + (page_head + h) * a.W + d;
-    T* __restrict__ mx = (T*)a.kmax + (page_head + h) * a.W + d;
-    const bool merge = seg.first > 0;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      float l = lo[i], u = hi[i];
+      // over the gw lanes of this chunk, then over the blocks (the first lane of a chunk's group is the same thread in all but a last,
+      // shorter block, whose predecessors' results it reads behind a barrier)
       for (int m = 1; m < gw; m <<= 1) {
-        l = smaller(l, __shfl_xor(l, m));
-        u = larger(u, __shfl_xor(u, m));
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          lo[i] = smaller(lo[i], __shfl_xor(lo[i], m));
+          hi[i] = larger(hi[i], __shfl_xor(hi[i], m));
+        }
       }
       if (gl == 0) {
-        if (merge) {
-          l = smaller(l, to_f(mn[i]));
-          u = larger(u, to_f(mx[i]));
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          s_lo[ch * VEC + i] = begun ? smaller(lo[i], s_lo[ch * VEC + i]) : lo[i];
+          s_hi[ch * VEC + i] = begun ? larger(hi[i], s_hi[ch * VEC + i]) : hi[i];
         }
-        mn[i] = (T)l;
-        mx[i] = (T)u;
       }
     }
+    begun = true;
+    __syncthreads();
+  }
+#pragma unroll
+  for (int j = 0; j < OLD; ++j) {
+    const int i = tid + 256 * j;
+    if (i >= nh * a.hd) break;
+    const long long at = (page_head + h0 + i / a.hd) * a.W + i % a.hd;
+    ((T*)a.kmin)[at] = (T)(merge ? smaller(s_lo[i], old_lo[j]) : s_lo[i]);
+    ((T*)a.kmax)[at] = (T)(merge ? larger(s_hi[i], old_hi[j]) : s_hi[i]);
   }
 }
 
@@ -614,47 +666,91 @@ __global__ __launch_bounds__(256) void k_paged_attention(AttArgs a) {
   }
 }
 
-// The join of a row's splits: one workgroup a row, 256 / (W / 4) splits at a time, sums in a fixed order.
+// The join of a row's splits.  Up to 64: a wave a row; lane s holds the weight of split s, W / 4 lanes a split's channels.
 template <class T, int W>
-__global__ __launch_bounds__(256) void k_paged_join(AttArgs a, int rows_per_block, int blocks) {
-  constexpr int L = W / 4, N = 256 / L;
-  __shared__ f32x4 s_o[N][L];
-  __shared__ float s_l[N];
-  const int r_in = blockIdx.x % a.rows, rest = blockIdx.x / a.rows;  // rest = unit without its row block
-  const int unit = rest * a.row_blocks + r_in / rows_per_block;
+__global__ __launch_bounds__(256) void k_paged_join(AttArgs a, int rows_per_block, int blocks, int rows) {
+  constexpr int L = W == 96 ? 32 : W / 4, N = 64 / L;  // lanes of a split, splits side by side
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (r >= rows) return;
+  const int r_in = r % a.rows, unit = r / a.rows * a.row_blocks + r_in / rows_per_block;
   const Unit u = unit_of(a, unit);
   const int chunk = split_chunk(u.n, a.splits);
   if (u.n <= chunk) return;
   const int ns = (u.n + chunk - 1) / chunk;
-  const float* ml = a.part + (long long)blocks * rows_per_block * W;
+  const float2* ml = reinterpret_cast<const float2*>(a.part + (long long)blocks * rows_per_block * W);
   const long long first = ((long long)unit * a.splits) * rows_per_block + r_in % rows_per_block;
-  float top = -FLT_MAX;
-  for (int s = threadIdx.x & 63; s < ns; s += 64) top = fmaxf(top, ml[(first + (long long)s * rows_per_block) * 2]);
+  const float2 mine = lane < ns ? ml[first + (long long)lane * rows_per_block] : float2{-FLT_MAX, 0.0f};
+  float top = mine.x;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-  const int c = threadIdx.x % L, n = threadIdx.x / L;
+  const float f = __builtin_amdgcn_exp2f(mine.x - top);
+  float sum = f * mine.y;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+  const int c = lane % L, n = lane / L;
   f32x4 acc = {0, 0, 0, 0};
-  float l = 0.0f;
-  if (n < N)
-    for (int s = n; s < ns; s += N) {
-      const long long slot = first + (long long)s * rows_per_block;
-      const float f = __builtin_amdgcn_exp2f(ml[slot * 2] - top);
-      l += f * ml[slot * 2 + 1];
-      acc += f * *reinterpret_cast<const f32x4*>(a.part + slot * W + 4 * c);
-    }
+  for (int s0 = 0; s0 < ns; s0 += N) {
+    const int s = min(s0 + n, ns - 1);
+    const float w = s0 + n < ns ? __shfl(f, s) : 0.0f;
+    if (W != 96 || c < W / 4) acc += w * *reinterpret_cast<const f32x4*>(a.part + (first + (long long)s * rows_per_block) * W + 4 * c);
+  }
+#pragma unroll
+  for (int d = L; d < 64; d <<= 1)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) acc[x] += __shfl_xor(acc[x], d);
+  if (n > 0) return;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  T* out = (T*)a.out + row_offset(a, u, r_in);
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    if (4 * c + x < a.hd) out[4 * c + x] = (T)(acc[x] * inv);
+}
+
+// More than 64: a workgroup a row; the weights are laid into LDS first, so that the reads of the partial results do not wait for each
+// other, and its groups of W / 4 threads take the splits in turn.  Sums in a fixed order in both.
+constexpr int kJoinSplits = 512;
+template <class T, int W>
+__global__ __launch_bounds__(512) void k_paged_join_many(AttArgs a, int rows_per_block, int blocks) {
+  constexpr int L = W / 4, N = 512 / L;
+  __shared__ f32x4 s_o[N][L];
+  __shared__ float s_w[kJoinSplits], s_top[8], s_sum[8];
+  const int r_in = blockIdx.x % a.rows, unit = blockIdx.x / a.rows * a.row_blocks + r_in / rows_per_block;
+  const Unit u = unit_of(a, unit);
+  const int chunk = split_chunk(u.n, a.splits);
+  if (u.n <= chunk) return;
+  const int ns = (u.n + chunk - 1) / chunk, tid = threadIdx.x;
+  const float2* ml = reinterpret_cast<const float2*>(a.part + (long long)blocks * rows_per_block * W);
+  const long long first = ((long long)unit * a.splits) * rows_per_block + r_in % rows_per_block;
+  const float2 mine = tid < ns ? ml[first + (long long)tid * rows_per_block] : float2{-FLT_MAX, 0.0f};
+  float top = mine.x;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+  if ((tid & 63) == 0) s_top[tid >> 6] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) top = fmaxf(top, s_top[w]);
+  const float f = __builtin_amdgcn_exp2f(mine.x - top);
+  s_w[tid] = f;
+  float l = f * mine.y;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
+  if ((tid & 63) == 0) s_sum[tid >> 6] = l;
+  __syncthreads();
+  const int c = tid % L, n = tid / L;
+  f32x4 acc = {0, 0, 0, 0};
   if (n < N) {
+#pragma unroll 8
+    for (int s = n; s < ns; s += N) acc += s_w[s] * *reinterpret_cast<const f32x4*>(a.part + (first + (long long)s * rows_per_block) * W + 4 * c);
     s_o[n][c] = acc;
-    if (c == 0) s_l[n] = l;
   }
   __syncthreads();
-  if (threadIdx.x < L) {
+  if (tid < L) {
     float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) sum += s_sum[w];
     f32x4 v = {0, 0, 0, 0};
 #pragma unroll 4
-    for (int i = 0; i < N; ++i) {
-      sum += s_l[i];
-      v += s_o[i][c];
-    }
+    for (int i = 0; i < N; ++i) v += s_o[i][c];
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     T* out = (T*)a.out + row_offset(a, u, r_in);
 #pragma unroll
@@ -676,8 +772,8 @@ struct SelectArgs {
   int* out;        // [B, T, H, count]
 };
 
-// One summary is read once: W / 8 lanes take 8 channels of a page each, 64 / that many pages side by side in a wave, two steps of them
-// at a time, all query rows over them.  The lanes' sums meet in a rotation within the 16-lane row, whose result is the same in
+// One summary is read once: W / 8 lanes take 8 channels of a page each, 64 / that many pages side by side in a wave, two such sets
+// at a time as 64-bit numbers in registers, all query rows over them.  The lanes' sums meet in a rotation within the 16-lane row, whose result is the same in
 // every lane.  (The 64-bit matrix instruction reaches 42 TFLOP/s here and pays for 16 rows whatever their number; four rows on
 // the vector unit cost less than the read.)
 template <int N>
@@ -703,96 +799,92 @@ __device__ __forceinline__ double group_sum(double x) {
   return x;
 }
 
-template <class T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  constexpr int N = 16 / sizeof(T);
-#pragma unroll
-  for (int i = 0; i < 8 / N; ++i) {
-    const Pack<T, N> v = reinterpret_cast<const Pack<T, N>*>(p)[i];
-#pragma unroll
-    for (int j = 0; j < N; ++j) x[N * i + j] = to_f(v.v[j]);
-  }
-}
-
-constexpr int kScoreRows = 4;  // query rows in registers at a time
-
-struct ScoreQuery {
-  double plus[kScoreRows][8], minus[kScoreRows][8];
-};
-template <class T>
-__device__ __forceinline__ void load_query(const SelectArgs& a, int b, int h, int r0, int rows, int c0, ScoreQuery& q) {
-#pragma unroll
-  for (int r = 0; r < kScoreRows; ++r) {
-    const int row = min(r0 + r, rows - 1);
-    const T* p = (const T*)a.q + (((long long)b * a.T + row / a.G) * a.heads + (long long)h * a.G + row % a.G) * a.hd;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const double x = c0 + j < a.hd ? (double)to_f(p[c0 + j]) : 0.0;
-      q.plus[r][j] = x > 0.0 ? x : (x != x ? x : 0.0);
-      q.minus[r][j] = x < 0.0 ? x : 0.0;
-    }
-  }
-}
+constexpr int kScorePages = 2;  // pages of a lane group at a time
+constexpr int kQueryRows = 8;   // query rows in LDS
 
 template <class T, int W>
 __global__ __launch_bounds__(256) void k_paged_score(SelectArgs a) {
-  constexpr int L = W == 96 ? 16 : W / 8, GP = 64 / L, STEP = 2 * GP;
+  constexpr int L = W == 96 ? 16 : W / 8, GP = 64 / L, NP = kScorePages, STEP = NP * GP, N = 16 / sizeof(T);
+  __shared__ double2 s_q[kQueryRows][8][L];  // {max(q, 0), min(q, 0)} of channel 8 l + j at [row][j][l]
   const int unit = blockIdx.x / a.score_blocks, block = blockIdx.x % a.score_blocks;
   const int h = unit % a.H, b = unit / a.H;
   const int P = 1 << a.pshift;
   const int np = (int)min((long long)a.slots, ((long long)max(a.lengths[b], 0) + P - 1) >> a.pshift);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c0 = (lane % L) * 8, gp = lane / L;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lc = lane % L, c0 = lc * 8, gp = lane / L;
   const int per_block = 4 * STEP * a.score_steps;
-  if (block * per_block >= np) return;
   const int rows = a.T * a.G;
-  ScoreQuery q;
-  load_query<T>(a, b, h, 0, rows, c0, q);
+  if (block * per_block >= np) return;
+  auto query = [&](int r0) {
+    const int n = min(kQueryRows, rows - r0) * 8 * L;
+    for (int i = threadIdx.x; i < n; i += 256) {
+      const int r = r0 + i / (8 * L), c = i % (8 * L);
+      float x = 0.0f;
+      if (c < a.hd) x = to_f(((const T*)a.q)[(((long long)b * a.T + r / a.G) * a.heads + (long long)h * a.G + r % a.G) * a.hd + c]);
+      s_q[i / (8 * L)][c % 8][c / 8] = double2{(double)(x < 0.0f ? 0.0f : x), (double)(x < 0.0f ? x : 0.0f)};  // (a NaN stays)
+    }
+  };
+  query(0);
+  __syncthreads();
+#pragma unroll 1
   for (int step = 0; step < a.score_steps; ++step) {
     const int first = block * per_block + (step * 4 + wave) * STEP;
-    if (first >= np) break;
-    double mx[2][8], mn[2][8];
-    bool there[2];
+    if (rows <= kQueryRows && first >= np) break;  // (with more rows the workgroup stays together: it loads them again)
+    double mx[NP][8], mn[NP][8];
+    int page[NP];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < NP; ++i) {
       const int slot = first + i * GP + gp;
-      const int page = slot < np ? a.table[(long long)b * a.slots + slot] : -1;
-      there[i] = page >= 0 && page < a.num_pages;
-      float x[8];
-      const long long at = ((long long)(there[i] ? page : 0) * a.H + h) * W + c0;
-      if (W != 96 || c0 < W) load8((const T*)a.kmax + at, x);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) mx[i][j] = W != 96 || c0 < W ? (double)x[j] : 0.0;
-      if (W != 96 || c0 < W) load8((const T*)a.kmin + at, x);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) mn[i][j] = W != 96 || c0 < W ? (double)x[j] : 0.0;
+      page[i] = a.table[(long long)b * a.slots + min(slot, np - 1)];
+      if (page[i] >= a.num_pages || slot >= np) page[i] = -1;
     }
-    double best[2] = {-INFINITY, -INFINITY};
-    for (int r0 = 0; r0 < rows; r0 += kScoreRows) {
-      if (rows > kScoreRows) load_query<T>(a, b, h, r0, rows, c0, q);
 #pragma unroll
-      for (int r = 0; r < kScoreRows; ++r) {
-        if (r0 + r >= rows) break;
+    for (int i = 0; i < NP; ++i) {
+      const long long at = ((long long)max(page[i], 0) * a.H + h) * W + (W == 96 ? min(c0, 88) : c0);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          double s = 0.0;
+      for (int j = 0; j < 8 / N; ++j) {
+        const Pack<T, N> hi = reinterpret_cast<const Pack<T, N>*>((const T*)a.kmax + at)[j];
+        const Pack<T, N> lo = reinterpret_cast<const Pack<T, N>*>((const T*)a.kmin + at)[j];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            s = fma(q.plus[r][j], mx[i][j], s);
-            s = fma(q.minus[r][j], mn[i][j], s);
-          }
-          s = group_sum<L>(s);
-          best[i] = (s > best[i] || s != s) ? s : best[i];
+        for (int x = 0; x < N; ++x) {
+          mx[i][N * j + x] = W != 96 || c0 < W ? (double)to_f(hi.v[x]) : 0.0;  // (lanes without channels)
+          mn[i][N * j + x] = W != 96 || c0 < W ? (double)to_f(lo.v[x]) : 0.0;
         }
-        const int row = r0 + r;
-        if (row % a.G == a.G - 1) {
-          const int t = row / a.G;
+      }
+    }
+    double best[NP];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int slot = first + i * GP + gp;
-            if (slot < np && lane % L == 0) a.scores[(((long long)b * a.T + t) * a.H + h) * a.slots + slot] = there[i] ? best[i] : -INFINITY;
-            best[i] = -INFINITY;
-          }
+    for (int i = 0; i < NP; ++i) best[i] = -INFINITY;
+    int g = 0, t = 0;
+#pragma unroll 1
+    for (int r = 0; r < rows; ++r) {
+      if (rows > kQueryRows && r % kQueryRows == 0) {
+        __syncthreads();
+        query(r);
+        __syncthreads();
+      }
+      double s[NP];
+#pragma unroll
+      for (int i = 0; i < NP; ++i) s[i] = 0.0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const double2 q = s_q[r % kQueryRows][j][lc];
+#pragma unroll
+        for (int i = 0; i < NP; ++i) s[i] = fma(q.y, mn[i][j], fma(q.x, mx[i][j], s[i]));
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const double x = group_sum<L>(s[i]);
+        best[i] = (x > best[i] || x != x) ? x : best[i];
+      }
+      if (++g == a.G) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const int slot = first + i * GP + gp;
+          if (slot < np && lc == 0) a.scores[(((long long)b * a.T + t) * a.H + h) * a.slots + slot] = page[i] >= 0 ? best[i] : -INFINITY;
+          best[i] = -INFINITY;
         }
+        g = 0;
+        ++t;
       }
     }
   }
@@ -806,177 +898,229 @@ __device__ __forceinline__ unsigned long long score_key(double s) {
 }
 constexpr unsigned long long kNotThere = 0x000fffffffffffffull;  // score_key(-inf)
 
-// The count best of a row, the lowest slots first among equals, written in ascending order.  A threshold bucket is found by histogram
-// over [smallest, largest] key of the candidates: first over the scores themselves (2048 equal steps: scores spread over them whatever
-// their scale), then, in the bucket that holds the border, over the keys as integers, each time from their highest differing bit: 11 bits
-// a pass, so it ends.  Then one ordered pass writes what lies above the bucket, and of the last bucket's equals the first `need`.
-constexpr int kBuckets = 2048;
+// The count best of a row, the lowest slots first among equals, written in ascending order.  The scores lie in LDS rounded to 32 bits (a monotone
+// map: they sort into buckets as the scores do; the part of a row behind CAP pages is read again in each pass); the scores themselves are
+// read again only where two of a bucket have to be told apart.  A histogram over 2048 equal steps between the smallest and the largest finds the bucket that holds the border;
+// up to kFew of a bucket are ranked against each other by score and slot.  A bucket with more (many near-equals, or a few scores far
+// from the rest) is divided again by the scores' bits as integers, from their highest differing bit: 11 bits a pass, so it ends.
+constexpr int kBuckets = 2048, kFew = 256;
+template <int CAP>
 __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
+  __shared__ float s_score[CAP];
   __shared__ int s_hist[kBuckets];
-  __shared__ unsigned long long s_lo[16], s_hi[16];
-  __shared__ int s_sum[16], s_bin, s_above;
-  __shared__ int s_wave[2][16];
+  __shared__ unsigned long long s_lo[16], s_hi[16], s_key[kFew], s_last_key;
+  __shared__ float s_f[2][16];
+  __shared__ int s_slot[kFew], s_sum[16], s_bin, s_above, s_few, s_last_slot;
   const long long row = blockIdx.x;
   const int b = (int)(row / ((long long)a.T * a.H));
   const double* __restrict__ sc = a.scores + row * a.slots;
   int* __restrict__ out = a.out + row * a.count;
-  const int P = 1 << a.pshift;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, P = 1 << a.pshift;
   const int np = (int)min((long long)a.slots, ((long long)max(a.lengths[b], 0) + P - 1) >> a.pshift);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  constexpr int R = 4;  // scores that a thread keeps (rows of up to 4096 pages are read once)
-  double mine[R];
+  // -inf: not there (a score below the range of 32 bits is its lowest value)
+  auto rounded = [](double s) { return s == -INFINITY ? -INFINITY : s < -(double)FLT_MAX ? -FLT_MAX : (float)s; };
+  const int kept = min(np, CAP);
+  for (int i0 = tid; i0 < kept; i0 += 8 * 1024) {
+    double x[8];
 #pragma unroll
-  for (int i = 0; i < R; ++i) mine[i] = tid + 1024 * i < np ? sc[tid + 1024 * i] : -INFINITY;
-  auto score = [&](int i) { return i < R ? (i == 0 ? mine[0] : i == 1 ? mine[1] : i == 2 ? mine[2] : mine[3]) : sc[tid + 1024 * i]; };
-  const int mine_n = np > tid ? (np - tid + 1023) / 1024 : 0;
+    for (int i = 0; i < 8; ++i) x[i] = sc[min(i0 + 1024 * i, a.slots - 1)];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i0 + 1024 * i < kept) s_score[i0 + 1024 * i] = rounded(x[i]);
+  }
+  for (int i = tid; i < kBuckets; i += 1024) s_hist[i] = 0;
+  __syncthreads();
+  // f(slot, rounded score) over the thread's slots
+  auto each = [&](auto f) {
+    for (int i = tid; i < kept; i += 1024) f(i, s_score[i]);
+    for (int i = tid + CAP; i < np; i += 1024) f(i, rounded(sc[i]));
+  };
 
-  // candidates: keys in [lo, hi]; everything above hi is taken
-  unsigned long long lo = kNotThere + 1, hi = ~0ull;
-  int need = a.count;
-  bool all = false, exact = false;
-  for (int pass = 0;; ++pass) {
-    unsigned long long mn = ~0ull, mx = 0;
-    int n = 0;
-    for (int i = 0; i < mine_n; ++i) {
-      const unsigned long long k = score_key(score(i));
-      if (k >= lo && k <= hi) {
-        mn = min(mn, k);
-        mx = max(mx, k);
-        ++n;
+  float flo = INFINITY, fhi = -INFINITY;
+  int n = 0;
+  each([&](int, float x) {
+    n += !(x == -INFINITY);
+    if (fabsf(x) < INFINITY) {
+      flo = fminf(flo, x);
+      fhi = fmaxf(fhi, x);
+    }
+  });
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    flo = fminf(flo, __shfl_xor(flo, d));
+    fhi = fmaxf(fhi, __shfl_xor(fhi, d));
+    n += __shfl_xor(n, d);
+  }
+  if (lane == 0) {
+    s_f[0][wave] = flo;
+    s_f[1][wave] = fhi;
+    s_sum[wave] = n;
+  }
+  __syncthreads();
+  n = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    flo = fminf(flo, s_f[0][w]);
+    fhi = fmaxf(fhi, s_f[1][w]);
+    n += s_sum[w];
+  }
+  // (where the step is infinite or no number -- no two finite scores -- all of them are in bucket 0)
+  const float inv = (float)(kBuckets - 1) / (fhi - flo);
+  auto bucket = [&](float x) {
+    if (x != x) return kBuckets - 1;
+    const float y = (x - flo) * inv;
+    return y >= (float)(kBuckets - 1) ? kBuckets - 1 : y > 0.0f ? (int)y : 0;
+  };
+  // buckets above `border` are taken, and of those in it what is above last_key, or equal to it with a slot up to last_slot
+  int border = -1, last_slot = 0x7fffffff;
+  unsigned long long last_key = 0;
+  if (n > a.count) {
+    int need = a.count;
+    unsigned long long lo = kNotThere + 1, hi = ~0ull;  // keys of the border bucket's candidates
+    int shift = -1;
+    // f(slot, key, part) over the candidates; part: the bucket of a later pass
+    auto candidates = [&](auto f) {
+      each([&](int slot, float x) {
+        if (x == -INFINITY || bucket(x) != border) return;
+        const unsigned long long k = score_key(sc[slot]);
+        if (k >= lo && k <= hi) f(slot, k);
+      });
+    };
+    each([&](int, float x) {
+      if (!(x == -INFINITY)) atomicAdd(&s_hist[bucket(x)], 1);
+    });
+    for (;;) {
+      if (tid == 0) s_few = 0;
+      __syncthreads();
+      // the bucket that holds the border: counts from the top, two buckets a thread
+      const int b1 = kBuckets - 1 - 2 * tid, h1 = s_hist[b1], h0 = s_hist[b1 - 1];
+      int upto = h1 + h0;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(upto, d);
+        if (lane >= d) upto += o;
       }
-    }
+      if (lane == 63) s_sum[wave] = upto;
+      __syncthreads();
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      mn = min(mn, (unsigned long long)__shfl_xor((long long)mn, d));
-      mx = max(mx, (unsigned long long)__shfl_xor((long long)mx, d));
-      n += __shfl_xor(n, d);
-    }
-    if (lane == 0) {
-      s_lo[wave] = mn;
-      s_hi[wave] = mx;
-      s_sum[wave] = n;
-    }
-    for (int i = tid; i < kBuckets; i += 1024) s_hist[i] = 0;
-    __syncthreads();
-    n = 0;
-#pragma unroll
-    for (int w = 0; w < 16; ++w) {
-      mn = min(mn, s_lo[w]);
-      mx = max(mx, s_hi[w]);
-      n += s_sum[w];
-    }
-    if (n <= need) {  // all candidates
-      all = true;
-      if (n > 0) lo = mn;
-      break;
-    }
-    lo = mn;
-    hi = mx;
-    if (mn == mx) {  // equals: the first `need` of them
-      exact = true;
-      break;
-    }
-    const unsigned long long kInfKey = 0xfff0000000000000ull, kLowKey = kNotThere + 1;
-    const bool linear = pass == 0 && mx < kInfKey && mn >= kLowKey;  // (finite scores)
-    const double base = linear ? __longlong_as_double((mn >> 63) ? (long long)(mn & 0x7fffffffffffffffull) : (long long)~mn) : 0.0;
-    const double top = linear ? __longlong_as_double((mx >> 63) ? (long long)(mx & 0x7fffffffffffffffull) : (long long)~mx) : 0.0;
-    const double inv = linear ? (double)(kBuckets - 1) / (top - base) : 0.0;
-    const int shift = max(0, 64 - __clzll((long long)(mx - mn)) - 11);
-    // (a step that is no number, or infinite: all in one bucket, and the next pass goes by the integers)
-    auto bucket = [&](double s, unsigned long long k) { return linear ? min(max((int)((s - base) * inv), 0), kBuckets - 1) : (int)((k - mn) >> shift); };
-    for (int i = 0; i < mine_n; ++i) {
-      const double s = score(i);
-      const unsigned long long k = score_key(s);
-      if (k >= lo && k <= hi) atomicAdd(&s_hist[bucket(s, k)], 1);
-    }
-    __syncthreads();
-    // the bucket that holds the border: counts from the top, two buckets a thread
-    const int b1 = kBuckets - 1 - 2 * tid, h1 = s_hist[b1], h0 = s_hist[b1 - 1];
-    int upto = h1 + h0;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(upto, d);
-      if (lane >= d) upto += o;
-    }
-    if (lane == 63) s_sum[wave] = upto;
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) upto += s_sum[w];
-    const int before = upto - h1 - h0;
-    if (before < need && upto >= need) {
-      s_bin = before + h1 >= need ? b1 : b1 - 1;
-      s_above = before + h1 >= need ? before : before + h1;
-    }
-    __syncthreads();
-    const int bin = s_bin;
-    need -= s_above;
-    // the bucket's own smallest and largest key are the next candidates' (found by the next pass's reduction)
-    unsigned long long bl = ~0ull, bh = 0;
-    for (int i = 0; i < mine_n; ++i) {
-      const double s = score(i);
-      const unsigned long long k = score_key(s);
-      if (k >= lo && k <= hi && bucket(s, k) == bin) {
+      for (int w = 0; w < 16; ++w) upto += w < wave ? s_sum[w] : 0;
+      const int before = upto - h1 - h0;
+      if (before < need && upto >= need) {
+        const bool upper = before + h1 >= need;
+        s_bin = upper ? b1 : b1 - 1;
+        s_above = upper ? before : before + h1;
+      }
+      __syncthreads();
+      const int bin = s_bin, inside = s_hist[bin];
+      need -= s_above;
+      if (shift < 0) {
+        border = bin;
+      } else {
+        const unsigned long long from = lo + ((unsigned long long)bin << shift);
+        hi = min(hi, from + ((1ull << shift) - 1));
+        lo = from;
+      }
+      if (inside <= kFew) {
+        candidates([&](int slot, unsigned long long k) {
+          const int at = atomicAdd(&s_few, 1);  // (any order: the ranks are of key and slot)
+          s_key[at] = k;
+          s_slot[at] = slot;
+        });
+        __syncthreads();
+        if (tid < inside) {
+          const unsigned long long k = s_key[tid];
+          const int slot = s_slot[tid];
+          int rank = 1;
+          for (int i = 0; i < inside; ++i) rank += s_key[i] > k || (s_key[i] == k && s_slot[i] < slot);
+          if (rank == need) {
+            s_last_key = k;
+            s_last_slot = slot;
+          }
+        }
+        __syncthreads();
+        last_key = s_last_key;
+        last_slot = s_last_slot;
+        break;
+      }
+      // the candidates' smallest and largest key
+      unsigned long long bl = ~0ull, bh = 0;
+      candidates([&](int, unsigned long long k) {
         bl = min(bl, k);
         bh = max(bh, k);
+      });
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        bl = min(bl, (unsigned long long)__shfl_xor((long long)bl, d));
+        bh = max(bh, (unsigned long long)__shfl_xor((long long)bh, d));
+      }
+      if (lane == 0) {
+        s_lo[wave] = bl;
+        s_hi[wave] = bh;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < 16; ++w) {
+        bl = min(bl, s_lo[w]);
+        bh = max(bh, s_hi[w]);
+      }
+      lo = bl;
+      hi = bh;
+      if (lo == hi) {  // many equals: the slot of the need-th of them
+        int base = 0;
+        for (int i0 = 0; i0 < np && base < need; i0 += 1024) {
+          const int slot = i0 + tid;
+          const bool is = slot < np && score_key(sc[slot]) == lo;
+          const unsigned long long m = __ballot(is);
+          __syncthreads();
+          if (lane == 0) s_sum[wave] = __popcll(m);
+          __syncthreads();
+          int at = base;
+#pragma unroll
+          for (int w = 0; w < 16; ++w) {
+            at += w < wave ? s_sum[w] : 0;
+            base += s_sum[w];
+          }
+          at += __popcll(m & ((1ull << lane) - 1));
+          if (is && at == need - 1) s_last_slot = slot;
+        }
+        __syncthreads();
+        last_key = lo;
+        last_slot = s_last_slot;
+        break;
+      }
+      shift = max(0, 64 - __clzll((long long)(hi - lo)) - 11);
+      for (int i = tid; i < kBuckets; i += 1024) s_hist[i] = 0;
+      __syncthreads();
+      candidates([&](int, unsigned long long k) { atomicAdd(&s_hist[(int)((k - lo) >> shift)], 1); });
+    }
+  }
+
+  int base = 0;
+  auto emit = [&](int slot, float x) {
+    bool take = slot < np && !(x == -INFINITY);
+    if (take && border >= 0) {
+      const int at = bucket(x);
+      take = at > border;
+      if (at == border) {
+        const unsigned long long k = score_key(sc[slot]);
+        take = k > last_key || (k == last_key && slot <= last_slot);
       }
     }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      bl = min(bl, (unsigned long long)__shfl_xor((long long)bl, d));
-      bh = max(bh, (unsigned long long)__shfl_xor((long long)bh, d));
-    }
+    const unsigned long long m = __ballot(take);
     __syncthreads();
-    if (lane == 0) {
-      s_lo[wave] = bl;
-      s_hi[wave] = bh;
-    }
+    if (lane == 0) s_sum[wave] = __popcll(m);
     __syncthreads();
+    int at = base;
 #pragma unroll
     for (int w = 0; w < 16; ++w) {
-      bl = min(bl, s_lo[w]);
-      bh = max(bh, s_hi[w]);
+      at += w < wave ? s_sum[w] : 0;
+      base += s_sum[w];
     }
-    lo = bl;
-    hi = bh;
-    __syncthreads();
-  }
-  // above hi: taken; in [lo, hi]: all of them, or the first `need`
-  int base_m = 0, base_t = 0;
-  for (int i = 0; i * 1024 < np; ++i) {
-    const int slot = i * 1024 + tid;
-    bool sure = false, maybe = false;
-    if (slot < np) {
-      const unsigned long long k = score_key(score(i));
-      if (k > kNotThere) {
-        sure = k > hi || (all && k >= lo);
-        maybe = exact && k == lo;
-      }
-    }
-    const unsigned long long below = (1ull << lane) - 1, bm = __ballot(maybe), bs = __ballot(sure);
-    if (lane == 0) {
-      s_wave[0][wave] = __popcll(bm);
-      s_wave[1][wave] = __popcll(bs);
-    }
-    __syncthreads();
-    int m = base_m, t = base_t, bm_all = 0, bs_all = 0;
-#pragma unroll
-    for (int w = 0; w < 16; ++w) {
-      if (w < wave) {
-        m += s_wave[0][w];
-        t += s_wave[1][w];
-      }
-      bm_all += s_wave[0][w];
-      bs_all += s_wave[1][w];
-    }
-    m += __popcll(bm & below);
-    t += __popcll(bs & below);
-    // (of the equals before this slot, those that were taken: the first `need`)
-    const int at = t + min(m, exact ? need : 0);
-    if ((sure || (maybe && m < need)) && at < a.count) out[at] = slot;
-    base_m += bm_all;
-    base_t += bs_all;
-    __syncthreads();
-  }
-  for (int i = base_t + min(base_m, exact ? need : 0) + tid; i < a.count; i += 1024) out[i] = -1;
+    at += __popcll(m & ((1ull << lane) - 1));
+    if (take && at < a.count) out[at] = slot;
+  };
+  for (int i = tid; i - tid < np; i += 1024) emit(i, i < kept ? s_score[i] : i < np ? rounded(sc[i]) : -INFINITY);
+  for (int i = base + tid; i < a.count; i += 1024) out[i] = -1;
 }
 
 template <class TI, class T, int VEC, int VT>
@@ -987,9 +1131,17 @@ void append_go(const AppendArgs& a, int units, hipStream_t s) {
 template <class TI, class T>
 void append_typed(AppendArgs& a, int units, hipStream_t s) {
   constexpr int VEC = 16 / sizeof(T), VT = VEC;  // 16-byte stores both ways
-  // wide loads need every chunk at a multiple of its size
-  const uintptr_t align = sizeof(TI) * VEC < 16 ? sizeof(TI) * VEC : 16;
-  const bool wide = a.hd % VEC == 0 && a.k_stride % VEC == 0 && a.v_stride % VEC == 0 && (uintptr_t)a.k % align == 0 && (uintptr_t)a.v % align == 0;
+  // wide loads need every chunk of the row at a multiple of its size, and rotation pairs that start at even channels of the row
+  const uintptr_t align = sizeof(TI) * VEC;
+  const bool wide = (a.H * a.hd) % VEC == 0 && a.k_stride % VEC == 0 && a.v_stride % VEC == 0 && (uintptr_t)a.k % align == 0 && (uintptr_t)a.v % align == 0 &&
+                    (a.rotary == 0 || a.rotary > a.hd || a.hd % 2 == 0);
+  // heads of a workgroup: as many workgroups as keep the chip busy, but not fewer than 128 chunks each (of a context's mean number of
+  // tokens); whole chunks, at most kAppendRow channels
+  const int step = wide ? VEC : 1, unit = step / std::gcd(a.hd, step);
+  const long long chunks = (long long)a.H * a.hd / step * std::max(1, a.n_tokens / a.B / VT > (1 << a.pshift) / VT ? (1 << a.pshift) / VT : a.n_tokens / a.B / VT);
+  const int parts = (int)std::max(1LL, std::min<long long>({a.H, 2048 / units, chunks / 128}));
+  a.heads_per_wg = std::min((a.H + parts - 1) / parts, std::max(1, kAppendRow / a.hd));
+  a.heads_per_wg = std::max(a.heads_per_wg / unit, 1) * unit;
   if (wide)
     append_go<TI, T, VEC, VT>(a, units, s);
   else
@@ -1001,7 +1153,8 @@ void attention_go(const AttArgs& a, int blocks, hipStream_t s) {
   k_paged_attention<T, W, RT><<<blocks, 256, 0, s>>>(a);
   if (a.splits > 1) {
     const int rows = blocks / a.splits / a.row_blocks * a.rows;
-    k_paged_join<T, W><<<rows, 256, 0, s>>>(a, 16 * RT, blocks);
+    if (a.splits <= 64) k_paged_join<T, W><<<(rows + 3) / 4, 256, 0, s>>>(a, 16 * RT, blocks, rows);
+    else k_paged_join_many<T, W><<<rows, 512, 0, s>>>(a, 16 * RT, blocks);
   }
 }
 template <class T>
@@ -1045,7 +1198,7 @@ AttPlan attention_plan(int B, int T, int H, int G, int W, long long capacity, bo
   p.row_blocks = (rows + 16 * p.RT - 1) / (16 * p.RT);
   p.units = (long long)B * (selected ? T : 1) * H * p.row_blocks;
   const long long most = std::max(1LL, (capacity + kMinChunk - 1) / kMinChunk);
-  p.splits = (int)std::min(most, std::max(1LL, kTargetWgs / std::max(1LL, p.units)));
+  p.splits = (int)std::min({most, (long long)kJoinSplits, std::max(1LL, kTargetWgs / std::max(1LL, p.units))});
   return p;
 }
 
@@ -1068,8 +1221,6 @@ int launch_paged_append(const void* k, long long k_stride, const void* v, long l
   a.keys = keys, a.values = values, a.kmin = kmin, a.kmax = kmax;
   // (context, page) pairs: each holds a token, and a context has at most two pages more than its tokens fill
   const int units = (int)std::min<long long>(n_tokens, (n_tokens >> pshift) + 2LL * B);
-  const int parts = std::min(H, std::max(1, 1024 / units));
-  a.heads_per_wg = (H + parts - 1) / parts;
   if (type == 0 && in_type == 0) append_typed<float, float>(a, units, s);
   else if (type == 1 && in_type == 0) append_typed<float, _Float16>(a, units, s);
   else if (type == 2 && in_type == 0) append_typed<float, __bf16>(a, units, s);
@@ -1112,7 +1263,7 @@ int launch_paged_select(const void* q, const void* kmin, const void* kmax, int t
   a.q = q, a.kmin = kmin, a.kmax = kmax, a.table = table, a.lengths = lengths;
   a.B = B, a.T = T, a.heads = H * G, a.H = H, a.G = G, a.hd = hd, a.W = paged_width(hd), a.slots = slots, a.num_pages = num_pages, a.pshift = pshift;
   a.count = count, a.scores = work, a.out = out;
-  const int L = a.W == 96 ? 16 : a.W / 8, per_step = 4 * 2 * (64 / L);  // pages of a workgroup's step
+  const int L = a.W == 96 ? 16 : a.W / 8, per_step = 4 * kScorePages * (64 / L);  // pages of a workgroup's step
   const long long all_steps = (long long)B * H * ((slots + per_step - 1) / per_step);
   a.score_steps = (int)std::min(16LL, std::max(1LL, all_steps / 2048));  // about 8 workgroups a CU, each with its query loaded once
   a.score_blocks = (slots + per_step * a.score_steps - 1) / (per_step * a.score_steps);
@@ -1121,7 +1272,9 @@ int launch_paged_select(const void* q, const void* kmin, const void* kmax, int t
   if (type == 0) score_typed<float>(a, blocks, s);
   else if (type == 1) score_typed<_Float16>(a, blocks, s);
   else score_typed<__bf16>(a, blocks, s);
-  k_paged_select<<<B * T * H, 1024, 0, s>>>(a);
+  // LDS for the row's scores: 16 KB leave room for two rows a CU, 128 KB hold rows of up to 32 768 pages
+  if (slots <= 4096) k_paged_select<4096><<<B * T * H, 1024, 0, s>>>(a);
+  else k_paged_select<32768><<<B * T * H, 1024, 0, s>>>(a);
   return 0;
 }
 
