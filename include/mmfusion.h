@@ -593,8 +593,8 @@ int mmf_attention_small(const float* q_dev, const float* k_dev, long long k_row_
 #define MMF_TYPE_F16 1
 #define MMF_TYPE_BF16 2
 int mmf_paged_width(int head_dim);
-/* Rows offsets[b] .. offsets[b + 1] - 1 of k and v ([tokens, kv_heads * head_dim], row strides in elements, last dimension contiguous;
- * the pages' type or float32) become tokens starts[b], starts[b] + 1, ... of context b; offsets [B + 1] int32 ascending, rows behind
+/* Rows offsets[b] .. offsets[b + 1] - 1 of k and v ([tokens, kv_heads * head_dim], row strides below 2^23 elements, last dimension
+ * contiguous; the pages' type or float32) become tokens starts[b], starts[b] + 1, ... of context b; offsets [B + 1] int32 ascending, rows behind
  * offsets[B] are not read; tokens beyond the table are not stored.  rotary_dim != 0: the keys' channel pairs (2 i, 2 i + 1) are rotated
  * on the way by positions [tokens, axes] (float32): the first rotary_dim channels of every head, or of the whole row if rotary_dim ==
  * kv_heads * head_dim; axis a has the channels [a, a + 1) * rotary_dim / axes, pair j of it turns by position_a * rotary_base^(-2 j axes /

@@ -582,6 +582,7 @@ const char* paged_shape_error(int type, int B, int slots, int page_size, int H, 
   if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1))) return "page_size is 16, 32, 64, 128 or 256";
   if (paged_width(head_dim) == 0) return "1 <= head_dim <= 256";
   if ((int64_t)slots * page_size > 0x7fffff00LL) return "slots * page_size passes 31 bits";
+  if ((int64_t)H * page_size * paged_width(head_dim) > (1 << 30)) return "a page passes 2^30 elements";
   return nullptr;
 }
 int page_shift(int page_size) { return __builtin_ctz((unsigned)page_size); }
@@ -604,7 +605,8 @@ int mmf_paged_append(const void* k, int64_t k_row_stride, const void* v, int64_t
       return paged_fail(name, "rotary_dim is a multiple of 2 * axes, at most head_dim or kv_heads * head_dim, with positions of 1 to 4 axes");
   }
   if (tokens == 0) return MMF_OK;
-  if (!k || !v || k_row_stride < 0 || v_row_stride < 0) return paged_fail(name, "null or negatively strided k / v");
+  if (!k || !v || k_row_stride < 0 || v_row_stride < 0 || k_row_stride >= (1 << 23) || v_row_stride >= (1 << 23))
+    return paged_fail(name, "k and v with row strides of 0 to 2^23 - 1 elements");
   if (launch_paged_append(k, k_row_stride, v, v_row_stride, in_type, (int)tokens, positions, rotary_dim ? axes : 1, rotary_dim, rotary_base, offsets,
                           starts, table, B, slots, page_shift(page_size), kv_heads, head_dim, num_pages, type, keys, values, key_min, key_max,
                           (hipStream_t)stream) != 0)

@@ -51,8 +51,8 @@ __device__ __forceinline__ T stored(float x) {
 }
 
 // the smaller / larger of two; NaN if either is (a page that holds a NaN key shows it)
-__device__ __forceinline__ float smaller(float a, float b) { return (b < a || b != b) ? b : a; }
-__device__ __forceinline__ float larger(float a, float b) { return (b > a || b != b) ? b : a; }
+__device__ __forceinline__ float smaller(float a, float b) { return __builtin_elementwise_minimum(a, b); }
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 // ---- append ---------------------------------------------------------------------------------------------------------------------------
 // Token i of the rows offsets[b] .. offsets[b + 1] - 1 becomes token starts[b] + i - offsets[b] of context b.  A workgroup owns one
@@ -61,7 +61,7 @@ __device__ __forceinline__ float larger(float a, float b) { return (b > a || b !
 // are transposed in its registers so that both stores are wide.
 struct AppendArgs {
   const void *k, *v;
-  long long k_stride, v_stride;
+  long long k_stride, v_stride;  // below 2^23
   const float* positions;
   int axes, rotary;   // rotary channels: of every head (rotary <= hd) or of the whole row
   double log2_base;
@@ -126,15 +126,17 @@ __device__ __forceinline__ bool find_segment(const AppendArgs& a, int unit, Segm
   return false;
 }
 
-// VEC > 1: VEC neighbouring channels of the row (of one head or of two), whose rotation pairs are the lane's own; VEC == 1: any layout,
-// the partner is read beside it.  The page is taken in blocks of tokens whose cos / sin fit into LDS: computed once for all
-// heads (of the row's own pairs where the code covers the whole row), which takes them out of the registers and off the 128-byte
-// lines that bound the kernel.
-constexpr int kAngles = 4096, kAppendRow = 1024;  // entries of the table; channels of a workgroup at most
-template <class TI, class T, int VEC, int VT>
+// A thread takes VEC channels of VT slots.  KIND 2: the heads are whole chunks, everything moves in 16-byte pieces; 1: chunks of the row
+// that may belong to two heads, whose rotation pairs are still the lane's own (the policy's heads of 15); 0: any layout, one channel,
+// its partner read beside it.  The page is taken in blocks of tokens whose cos / sin fit into LDS: computed once for all heads (of the row's
+// own pairs where the code covers the whole row), at [slot of a group][chunk of pairs][group], the order in which lanes read them.
+constexpr int kAppendRow = 1024;  // channels of a workgroup at most
+template <class TI, class T, int KIND>
 __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
-  __shared__ float2 s_angle[kAngles];               // [token of the block][pair]: cos, sin
-  __shared__ double s_turns[kAppendRow / 2];        // turns a unit of position, by pair
+  constexpr int VT = 16 / sizeof(T), VEC = KIND ? VT : 1, NP = VEC > 1 ? VEC / 2 : 1;
+  constexpr int kAngles = sizeof(T) == 4 ? 2048 : 4096;  // (the 32-bit kernels have the registers for more workgroups a CU than 32 KB leave room for)
+  __shared__ __attribute__((aligned(16))) float2 s_angle[kAngles];
+  __shared__ double s_turns[kAppendRow / 2 + 8];    // turns a unit of position, by pair
   __shared__ float s_lo[kAppendRow], s_hi[kAppendRow];
   Segment seg;
   if (!find_segment(a, blockIdx.x, seg)) return;
@@ -147,14 +149,18 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
   const int pairs = a.rotary ? (whole_row ? (nh * a.hd + 1 + (c0 & 1)) / 2 : a.rotary / 2) : 0;  // (a whole row's pairs may begin before h0's first channel)
   const int pair0 = whole_row ? c0 / 2 : 0;
   const int span = a.rotary ? a.rotary / a.axes : 2;
-  const TI* __restrict__ kin = (const TI*)a.k;
-  const TI* __restrict__ vin = (const TI*)a.v;
+  // (bases that are the workgroup's, 32-bit offsets from them: the host checks that a page and 256 rows stay below 2^31 elements)
+  const TI* __restrict__ kin = (const TI*)a.k + (long long)seg.row * a.k_stride;
+  const TI* __restrict__ vin = (const TI*)a.v + (long long)seg.row * a.v_stride;
   const long long page_head = (long long)page * a.H;
+  T* __restrict__ kpage = (T*)a.keys + (page_head << a.pshift) * a.W;
+  T* __restrict__ vpage = (T*)a.values + (page_head << a.pshift) * a.W;
   for (int i = tid; i < pairs; i += 256) {
     const int j = (2 * (pair0 + i)) % span;  // pair j / 2 of its axis: position * base^(-j / span) / 2 pi turns
     s_turns[i] = exp2(-a.log2_base * (double)j / (double)span) * 0.15915494309189533576888;
   }
-  const int block = pairs ? min(256, kAngles / pairs / VT * VT) : 256;  // tokens of a block
+  const int pair_chunks = (pairs + NP - 1) / NP;
+  const int groups = pairs ? min(256 / VT, kAngles / (pair_chunks * NP * VT)) : 256 / VT, block = groups * VT;  // of a block
   // what the page's summary held (it begins anew with its first slot), asked for early: the first access to a page of a large pool waits long
   constexpr int OLD = kAppendRow / 256;
   const bool merge = seg.first > 0;
@@ -175,13 +181,13 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
       __syncthreads();
       const int n = (hi_slot - lo_slot) * pairs;
       for (int i = tid; i < n; i += 256) {
-        const int t = i / pairs, w = i - t * pairs, axis = 2 * (pair0 + w) / span;
+        const int t = i / pairs, w = i - t * pairs, axis = 2 * (pair0 + w) / span, at = lo_slot + t - first;
         const long long row = seg.row + (lo_slot + t - seg.first);
         // taken in turns and reduced in 64 bits (a far position times a frequency loses its fraction in 32), then in 32 on [-1/2, 1/2]
         const double turns = (double)a.positions[row * a.axes + axis] * s_turns[w];
         float2 cs;
         sincospif(2.0f * (float)(turns - rint(turns)), &cs.y, &cs.x);
-        s_angle[(lo_slot + t - first) * pairs + w] = cs;
+        s_angle[((at % VT * pair_chunks + w / NP) * groups + at / VT) * NP + w % NP] = cs;
       }
       __syncthreads();
     }
@@ -192,7 +198,20 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
     for (int ch = tid / gw; ch < nchunks; ch += 256 / gw) {
       const int c = c0 + ch * VEC;  // channel in the row
       const int h = c / a.hd, d = c - h * a.hd;
-      const bool one_head = d + VEC <= a.hd;
+      const bool one_head = KIND != 1 || d + VEC <= a.hd;
+      unsigned kat[VEC], vat[VEC];  // where slot 0 of channel c + i is in the page's keys and values
+      int pair[NP];                 // its pair in the table, or -1
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const int over = KIND == 1 && d + i >= a.hd ? (d + i) / a.hd : 0;
+        const int hh = h + over, dd = d + i - over * a.hd;
+        kat[i] = ((unsigned)hh << a.pshift) * a.W + dd;
+        vat[i] = ((unsigned)hh * a.W + dd) << a.pshift;
+        if (i % 2 == 0) {
+          const int w = whole_row ? c + i : dd;
+          pair[i / 2] = w < a.rotary ? w / 2 - pair0 : -1;
+        }
+      }
       float lo[VEC], hi[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
@@ -206,74 +225,81 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
         Pack<TI, VEC> kr[VT], vr[VT];
 #pragma unroll
         for (int t = 0; t < VT; ++t) {
-          const long long row = (long long)seg.row + (min(max(slot0 + t, lo_slot), hi_slot - 1) - seg.first);
-          kr[t] = *reinterpret_cast<const Pack<TI, VEC>*>(kin + row * a.k_stride + c);
-          vr[t] = *reinterpret_cast<const Pack<TI, VEC>*>(vin + row * a.v_stride + c);
+          const unsigned row = min(max(slot0 + t, lo_slot), hi_slot - 1) - seg.first;
+          kr[t] = *reinterpret_cast<const Pack<TI, VEC>*>(kin + (row * (unsigned)a.k_stride + (unsigned)c));
+          vr[t] = *reinterpret_cast<const Pack<TI, VEC>*>(vin + (row * (unsigned)a.v_stride + (unsigned)c));
         }
+        Pack<T, VEC> out[VT];
 #pragma unroll
         for (int t = 0; t < VT; ++t) {
-          const int slot = min(max(slot0 + t, lo_slot), hi_slot - 1);
+          const int slot = min(max(slot0 + t, lo_slot), hi_slot - 1), at = slot - first;
           float x[VEC];
 #pragma unroll
           for (int i = 0; i < VEC; ++i) x[i] = to_f(kr[t].v[i]);
           if (pairs) {
-            const float2* angle = s_angle + (slot - first) * pairs;
+            const float2* angle = s_angle + ((at % VT) * pair_chunks * groups + at / VT) * NP;
             if constexpr (VEC > 1) {
+              // (branch-free: a pair that is not turned reads some angle and keeps its values)
+              Pack<float2, NP> cs;
+              if (KIND == 2 || whole_row) {
+                cs = *reinterpret_cast<const Pack<float2, NP>*>(angle + max(pair[0], 0) / NP * groups * NP);
+              } else {
 #pragma unroll
-              for (int i = 0; i < VEC / 2; ++i) {
-                const int w = whole_row ? c + 2 * i : one_head ? d + 2 * i : (c + 2 * i) % a.hd;
-                if (w < a.rotary) {
-                  const float2 cs = angle[w / 2 - pair0];
-                  const float e = x[2 * i], o = x[2 * i + 1];
-                  x[2 * i] = e * cs.x - o * cs.y;
-                  x[2 * i + 1] = o * cs.x + e * cs.y;
-                }
+                for (int i = 0; i < NP; ++i) cs.v[i] = angle[max(pair[i], 0) / NP * groups * NP + max(pair[i], 0) % NP];
               }
-            } else {
-              const int w = whole_row ? c : d;
-              if (w < a.rotary) {
-                const float2 cs = angle[w / 2 - pair0];
-                const long long row = (long long)seg.row + (slot - seg.first);
-                const float p = to_f(kin[row * a.k_stride + c + ((w & 1) ? -1 : 1)]);
-                x[0] = (w & 1) ? x[0] * cs.x + p * cs.y : x[0] * cs.x - p * cs.y;
+#pragma unroll
+              for (int i = 0; i < NP; ++i) {
+                const float e = x[2 * i], o = x[2 * i + 1];
+                const float p = e * cs.v[i].x - o * cs.v[i].y, q = o * cs.v[i].x + e * cs.v[i].y;
+                x[2 * i] = pair[i] >= 0 ? p : e;
+                x[2 * i + 1] = pair[i] >= 0 ? q : o;
               }
+            } else if (pair[0] >= 0) {
+              const bool odd = (whole_row ? c : d) & 1;
+              const float2 cs = angle[pair[0] * groups];
+              const float p = to_f(kin[(unsigned)(slot - seg.first) * (unsigned)a.k_stride + (unsigned)c + (odd ? -1 : 1)]);
+              x[0] = odd ? x[0] * cs.x + p * cs.y : x[0] * cs.x - p * cs.y;
             }
           }
-          Pack<T, VEC> out;
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
-            out.v[i] = stored<T>(x[i]);  // the one rounding of a key; the summary is of the stored value
-            const float y = to_f(out.v[i]);
+            out[t].v[i] = stored<T>(x[i]);  // the one rounding of a key; the summary is of the stored value
+            const float y = to_f(out[t].v[i]);
             lo[i] = smaller(lo[i], y);
             hi[i] = larger(hi[i], y);
           }
-          if (full || slot == slot0 + t) {
-            T* kp = (T*)a.keys + ((page_head + h) << a.pshift) * a.W + (long long)slot * a.W + d;
-            if (one_head) {
-              *reinterpret_cast<Loose<T, VEC>*>(kp) = __builtin_bit_cast(Loose<T, VEC>, out);  // (16 bytes, aligned like the type)
+        }
+        if (full) {
+#pragma unroll
+          for (int t = 0; t < VT; ++t) {
+            T* to = kpage + ((unsigned)(slot0 + t) * a.W + kat[0]);
+            if (KIND == 2) {
+              *reinterpret_cast<Pack<T, VEC>*>(to) = out[t];
+            } else if (one_head) {
+              *reinterpret_cast<Loose<T, VEC>*>(to) = __builtin_bit_cast(Loose<T, VEC>, out[t]);  // (16 bytes, aligned like the type)
             } else {
 #pragma unroll
-              for (int i = 0; i < VEC; ++i) {
-                const int hh = (c + i) / a.hd, dd = (c + i) % a.hd;
-                ((T*)a.keys)[((page_head + hh) << a.pshift) * a.W + (long long)slot * a.W + dd] = out.v[i];
-              }
+              for (int i = 0; i < VEC; ++i) kpage[(unsigned)(slot0 + t) * a.W + kat[i]] = out[t].v[i];
             }
           }
-        }
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const int hh = one_head ? h : (c + i) / a.hd, dd = one_head ? d + i : (c + i) % a.hd;
-          T* vp = (T*)a.values + (((page_head + hh) * a.W + dd) << a.pshift) + slot0;
-          Pack<T, VT> out;
+          for (int i = 0; i < VEC; ++i) {
+            Pack<T, VT> col;
 #pragma unroll
-          for (int t = 0; t < VT; ++t) out.v[t] = (T)to_f(vr[t].v[i]);
-          if (full) {
-            *reinterpret_cast<Pack<T, VT>*>(vp) = out;
-          } else {
-#pragma unroll
-            for (int t = 0; t < VT; ++t)
-              if (slot0 + t >= lo_slot && slot0 + t < hi_slot) vp[t] = out.v[t];
+            for (int t = 0; t < VT; ++t) col.v[t] = (T)to_f(vr[t].v[i]);
+            *reinterpret_cast<Pack<T, VT>*>(vpage + (vat[i] + (unsigned)slot0)) = col;
           }
+        } else {
+#pragma unroll
+          for (int t = 0; t < VT; ++t)
+            if (slot0 + t >= lo_slot && slot0 + t < hi_slot) {
+              if (KIND == 2) *reinterpret_cast<Pack<T, VEC>*>(kpage + ((unsigned)(slot0 + t) * a.W + kat[0])) = out[t];
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) {
+                if (KIND != 2) kpage[(unsigned)(slot0 + t) * a.W + kat[i]] = out[t].v[i];
+                vpage[vat[i] + (unsigned)(slot0 + t)] = (T)to_f(vr[t].v[i]);
+              }
+            }
         }
       }
       // over the gw lanes of this chunk, then over the blocks (the first lane of a chunk's group is the same thread in all but a last,
@@ -393,6 +419,8 @@ __global__ __launch_bounds__(256) void k_paged_attention(AttArgs a) {
   constexpr int NC = W / 16;                                     // channel tiles
   constexpr int NQ = F32 ? W / 16 : (W >= 32 ? W / 32 : 1);      // key-row operands per 16 keys
   constexpr int ROWS = 16 * RT;
+  constexpr int NV = NC * (F32 ? 2 : 1);                          // 16-byte value loads of a tile
+  constexpr bool EARLY = NV * RT <= 8;
   __shared__ int s_page[kWindow], s_valid[kWindow];
   __shared__ float s_m[4][ROWS], s_l[4][ROWS];
   __shared__ float s_o[2][ROWS][W + 4];
@@ -459,6 +487,17 @@ __global__ __launch_bounds__(256) void k_paged_attention(AttArgs a) {
       // this lane's key row and value group; a group of 8 (4) keys lies in one page
       f32x4 s[RT][2];
       int left[2];  // valid keys of the lane's score group(s)
+      // the values' loads go out with the keys', where there are registers for both
+      uint4 early[EARLY ? NV : 1];
+      if constexpr (EARLY) {
+#pragma unroll
+        for (int t = 0; t < (F32 ? 2 : 1); ++t) {
+          const int i = base + (F32 ? 16 * t : 8 * g), e = min((i >> a.pshift) - e0, ne - 1);
+          const T* vr = values + s_page[e] * page_stride + (long long)r16 * P + (i & (P - 1)) + (F32 ? 4 * g : 0);
+#pragma unroll
+          for (int c = 0; c < NC; ++c) early[t * NC + c] = *reinterpret_cast<const uint4*>(vr + (long long)16 * c * P);
+        }
+      }
       if constexpr (F32) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -551,7 +590,7 @@ __global__ __launch_bounds__(256) void k_paged_attention(AttArgs a) {
           const T* vr = values + s_page[e] * page_stride + (long long)r16 * P + off;
 #pragma unroll
           for (int c = 0; c < NC; ++c) {
-            f32x4 vf = *reinterpret_cast<const f32x4*>(vr + (long long)16 * c * P);
+            f32x4 vf = EARLY ? __builtin_bit_cast(f32x4, early[EARLY ? t * NC + c : 0]) : *reinterpret_cast<const f32x4*>(vr + (long long)16 * c * P);
             if (ragged) {
 #pragma unroll
               for (int x = 0; x < 4; ++x) vf[x] = x < left[t] ? vf[x] : 0.0f;  // a weight of zero does not hide a NaN
@@ -579,7 +618,7 @@ __global__ __launch_bounds__(256) void k_paged_attention(AttArgs a) {
         const T* vr = values + s_page[ev] * page_stride + (long long)r16 * P + (iv & (P - 1));
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          typename Mma<T>::V8 vf = __builtin_bit_cast(typename Mma<T>::V8, *reinterpret_cast<const uint4*>(vr + (long long)16 * c * P));
+          typename Mma<T>::V8 vf = __builtin_bit_cast(typename Mma<T>::V8, EARLY ? early[EARLY ? c : 0] : *reinterpret_cast<const uint4*>(vr + (long long)16 * c * P));
           if (ragged) {
 #pragma unroll
             for (int x = 0; x < 8; ++x) vf[x] = x < left[0] ? vf[x] : (T)0.0f;
@@ -898,15 +937,15 @@ __device__ __forceinline__ unsigned long long score_key(double s) {
 }
 constexpr unsigned long long kNotThere = 0x000fffffffffffffull;  // score_key(-inf)
 
-// The count best of a row, the lowest slots first among equals, written in ascending order.  The scores lie in LDS rounded to 32 bits (a monotone
-// map: they sort into buckets as the scores do; the part of a row behind CAP pages is read again in each pass); the scores themselves are
-// read again only where two of a bucket have to be told apart.  A histogram over 2048 equal steps between the smallest and the largest finds the bucket that holds the border;
+// The count best of a row, the lowest slots first among equals, written in ascending order.  The scores are rounded to 32 bits (a monotone map: they
+// sort into buckets as the scores do) and their buckets kept in LDS (the part of a row behind CAP pages is read again in each pass); the
+// scores themselves are read again only where two of a bucket have to be told apart.  A histogram over 2048 equal steps between the smallest and the largest finds the bucket that holds the border;
 // up to kFew of a bucket are ranked against each other by score and slot.  A bucket with more (many near-equals, or a few scores far
 // from the rest) is divided again by the scores' bits as integers, from their highest differing bit: 11 bits a pass, so it ends.
 constexpr int kBuckets = 2048, kFew = 256;
 template <int CAP>
 __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
-  __shared__ float s_score[CAP];
+  __shared__ int s_bucket[CAP];
   __shared__ int s_hist[kBuckets];
   __shared__ unsigned long long s_lo[16], s_hi[16], s_key[kFew], s_last_key;
   __shared__ float s_f[2][16];
@@ -920,31 +959,30 @@ __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
   // -inf: not there (a score below the range of 32 bits is its lowest value)
   auto rounded = [](double s) { return s == -INFINITY ? -INFINITY : s < -(double)FLT_MAX ? -FLT_MAX : (float)s; };
   const int kept = min(np, CAP);
-  for (int i0 = tid; i0 < kept; i0 += 8 * 1024) {
-    double x[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = sc[min(i0 + 1024 * i, a.slots - 1)];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i0 + 1024 * i < kept) s_score[i0 + 1024 * i] = rounded(x[i]);
-  }
-  for (int i = tid; i < kBuckets; i += 1024) s_hist[i] = 0;
-  __syncthreads();
-  // f(slot, rounded score) over the thread's slots
-  auto each = [&](auto f) {
-    for (int i = tid; i < kept; i += 1024) f(i, s_score[i]);
-    for (int i = tid + CAP; i < np; i += 1024) f(i, rounded(sc[i]));
-  };
-
+  constexpr int AT_ONCE = CAP > 4096 ? 16 : 4;
   float flo = INFINITY, fhi = -INFINITY;
   int n = 0;
-  each([&](int, float x) {
+  auto meet = [&](float x) {
     n += !(x == -INFINITY);
     if (fabsf(x) < INFINITY) {
       flo = fminf(flo, x);
       fhi = fmaxf(fhi, x);
     }
-  });
+  };
+  for (int i0 = tid; i0 < kept; i0 += AT_ONCE * 1024) {
+    double x[AT_ONCE];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) x[i] = sc[min(i0 + 1024 * i, a.slots - 1)];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i)
+      if (i0 + 1024 * i < kept) {
+        const float y = rounded(x[i]);
+        s_bucket[i0 + 1024 * i] = __float_as_int(y);
+        meet(y);
+      }
+  }
+  for (int i = tid + CAP; i < np; i += 1024) meet(rounded(sc[i]));
+  for (int i = tid; i < kBuckets; i += 1024) s_hist[i] = 0;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     flo = fminf(flo, __shfl_xor(flo, d));
@@ -964,13 +1002,23 @@ __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
     fhi = fmaxf(fhi, s_f[1][w]);
     n += s_sum[w];
   }
-  // (where the step is infinite or no number -- no two finite scores -- all of them are in bucket 0)
+  // The bucket of a score, -1: not there.  (Where the step is infinite or no number -- no two finite scores -- all of them are in bucket 0.)
   const float inv = (float)(kBuckets - 1) / (fhi - flo);
   auto bucket = [&](float x) {
+    if (x == -INFINITY) return -1;
     if (x != x) return kBuckets - 1;
     const float y = (x - flo) * inv;
     return y >= (float)(kBuckets - 1) ? kBuckets - 1 : y > 0.0f ? (int)y : 0;
   };
+  for (int i = tid; i < kept; i += 1024) {
+    const int at = bucket(__int_as_float(s_bucket[i]));
+    s_bucket[i] = at;
+    if (at >= 0) atomicAdd(&s_hist[at], 1);
+  }
+  for (int i = tid + CAP; i < np; i += 1024) {
+    const int at = bucket(rounded(sc[i]));
+    if (at >= 0) atomicAdd(&s_hist[at], 1);
+  }
   // buckets above `border` are taken, and of those in it what is above last_key, or equal to it with a slot up to last_slot
   int border = -1, last_slot = 0x7fffffff;
   unsigned long long last_key = 0;
@@ -978,17 +1026,17 @@ __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
     int need = a.count;
     unsigned long long lo = kNotThere + 1, hi = ~0ull;  // keys of the border bucket's candidates
     int shift = -1;
-    // f(slot, key, part) over the candidates; part: the bucket of a later pass
+    // f(slot, key) over the candidates
     auto candidates = [&](auto f) {
-      each([&](int slot, float x) {
-        if (x == -INFINITY || bucket(x) != border) return;
+      auto one = [&](int slot) {
         const unsigned long long k = score_key(sc[slot]);
         if (k >= lo && k <= hi) f(slot, k);
-      });
+      };
+      for (int i = tid; i < kept; i += 1024)
+        if (s_bucket[i] == border) one(i);
+      for (int i = tid + CAP; i < np; i += 1024)
+        if (bucket(rounded(sc[i])) == border) one(i);
     };
-    each([&](int, float x) {
-      if (!(x == -INFINITY)) atomicAdd(&s_hist[bucket(x)], 1);
-    });
     for (;;) {
       if (tid == 0) s_few = 0;
       __syncthreads();
@@ -1095,57 +1143,56 @@ __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
     }
   }
 
-  int base = 0;
-  auto emit = [&](int slot, float x) {
-    bool take = slot < np && !(x == -INFINITY);
-    if (take && border >= 0) {
-      const int at = bucket(x);
-      take = at > border;
-      if (at == border) {
-        const unsigned long long k = score_key(sc[slot]);
-        take = k > last_key || (k == last_key && slot <= last_slot);
-      }
-    }
-    const unsigned long long m = __ballot(take);
-    __syncthreads();
-    if (lane == 0) s_sum[wave] = __popcll(m);
-    __syncthreads();
-    int at = base;
-#pragma unroll
-    for (int w = 0; w < 16; ++w) {
-      at += w < wave ? s_sum[w] : 0;
-      base += s_sum[w];
-    }
-    at += __popcll(m & ((1ull << lane) - 1));
-    if (take && at < a.count) out[at] = slot;
+  // a wave takes a run of slots: counted, then written behind the waves before it
+  auto taken = [&](int slot) {
+    if (slot >= np) return false;
+    const int at = slot < kept ? s_bucket[slot] : bucket(rounded(sc[slot]));
+    if (at != border) return at > border;
+    if (at < 0) return false;
+    const unsigned long long k = score_key(sc[slot]);
+    return k > last_key || (k == last_key && slot <= last_slot);
   };
-  for (int i = tid; i - tid < np; i += 1024) emit(i, i < kept ? s_score[i] : i < np ? rounded(sc[i]) : -INFINITY);
+  const int run = ((np + 15) / 16 + 63) & ~63, from = wave * run, to = min(np, from + run);
+  int mine = 0;
+  for (int i = from; i < to; i += 64) mine += __popcll(__ballot(taken(i + lane) && i + lane < to));
+  __syncthreads();  // (s_sum's last readers)
+  if (lane == 0) s_sum[wave] = mine;
+  __syncthreads();
+  int base = 0, before = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    before += w < wave ? s_sum[w] : 0;
+    base += s_sum[w];
+  }
+  for (int i = from; i < to; i += 64) {
+    const bool take = taken(i + lane) && i + lane < to;
+    const unsigned long long m = __ballot(take);
+    const int at = before + __popcll(m & ((1ull << lane) - 1));
+    if (take && at < a.count) out[at] = i + lane;
+    before += __popcll(m);
+  }
   for (int i = base + tid; i < a.count; i += 1024) out[i] = -1;
-}
-
-template <class TI, class T, int VEC, int VT>
-void append_go(const AppendArgs& a, int units, hipStream_t s) {
-  k_paged_append<TI, T, VEC, VT><<<dim3(units, (a.H + a.heads_per_wg - 1) / a.heads_per_wg), 256, 0, s>>>(a);
 }
 
 template <class TI, class T>
 void append_typed(AppendArgs& a, int units, hipStream_t s) {
-  constexpr int VEC = 16 / sizeof(T), VT = VEC;  // 16-byte stores both ways
-  // wide loads need every chunk of the row at a multiple of its size, and rotation pairs that start at even channels of the row
+  constexpr int VEC = 16 / sizeof(T);  // 16-byte stores both ways
+  // wide loads need whole chunks in a workgroup's heads, every chunk of the row at a multiple of its size, and rotation pairs that start at even channels of the row
   const uintptr_t align = sizeof(TI) * VEC;
-  const bool wide = (a.H * a.hd) % VEC == 0 && a.k_stride % VEC == 0 && a.v_stride % VEC == 0 && (uintptr_t)a.k % align == 0 && (uintptr_t)a.v % align == 0 &&
+  const bool wide = VEC / std::gcd(a.hd, VEC) * a.hd <= kAppendRow && (a.H * a.hd) % VEC == 0 && a.k_stride % VEC == 0 && a.v_stride % VEC == 0 && (uintptr_t)a.k % align == 0 && (uintptr_t)a.v % align == 0 &&
                     (a.rotary == 0 || a.rotary > a.hd || a.hd % 2 == 0);
   // heads of a workgroup: as many workgroups as keep the chip busy, but not fewer than 128 chunks each (of a context's mean number of
   // tokens); whole chunks, at most kAppendRow channels
   const int step = wide ? VEC : 1, unit = step / std::gcd(a.hd, step);
-  const long long chunks = (long long)a.H * a.hd / step * std::max(1, a.n_tokens / a.B / VT > (1 << a.pshift) / VT ? (1 << a.pshift) / VT : a.n_tokens / a.B / VT);
+  const int groups = std::max(1, std::min(a.n_tokens / a.B, 1 << a.pshift) / VEC);
+  const long long chunks = (long long)a.H * a.hd / step * groups;
   const int parts = (int)std::max(1LL, std::min<long long>({a.H, 2048 / units, chunks / 128}));
   a.heads_per_wg = std::min((a.H + parts - 1) / parts, std::max(1, kAppendRow / a.hd));
   a.heads_per_wg = std::max(a.heads_per_wg / unit, 1) * unit;
-  if (wide)
-    append_go<TI, T, VEC, VT>(a, units, s);
-  else
-    append_go<TI, T, 1, VT>(a, units, s);
+  const dim3 grid(units, (a.H + a.heads_per_wg - 1) / a.heads_per_wg);
+  if (wide && a.hd % VEC == 0) k_paged_append<TI, T, 2><<<grid, 256, 0, s>>>(a);
+  else if (wide) k_paged_append<TI, T, 1><<<grid, 256, 0, s>>>(a);
+  else k_paged_append<TI, T, 0><<<grid, 256, 0, s>>>(a);
 }
 
 template <class T, int W, int RT>
@@ -1189,16 +1236,18 @@ struct AttPlan {
   long long units;
   int row_blocks, splits, RT;
 };
-// Workgroups for 256 CUs: a unit's keys are split until there are about kTargetWgs of them, kMinChunk keys each at least.
-constexpr int kTargetWgs = 2048;
+// Workgroups for 256 CUs: a unit's keys are split until there are about 2048 (contexts are of unlike length: small pieces even that out;
+// 1024 took 291 us for 64 contexts of up to 8191 tokens, 2048 274, 4096 283), or 512 over selected pages, which are as many for each (119
+// against 112 us for 16 contexts x 64 pages of 64).  Up to 1024 keys are not split: the join costs what the split saves.
+constexpr int kTargetWgs = 2048, kTargetSelected = 512, kAlone = 1024;
 AttPlan attention_plan(int B, int T, int H, int G, int W, long long capacity, bool selected) {
   AttPlan p;
   const int rows = selected ? G : T * G;
   p.RT = row_tiles(rows, W);
   p.row_blocks = (rows + 16 * p.RT - 1) / (16 * p.RT);
   p.units = (long long)B * (selected ? T : 1) * H * p.row_blocks;
-  const long long most = std::max(1LL, (capacity + kMinChunk - 1) / kMinChunk);
-  p.splits = (int)std::min({most, (long long)kJoinSplits, std::max(1LL, kTargetWgs / std::max(1LL, p.units))});
+  const long long most = capacity <= kAlone ? 1 : (capacity + kMinChunk - 1) / kMinChunk;
+  p.splits = (int)std::min({most, (long long)kJoinSplits, std::max(1LL, (selected ? kTargetSelected : kTargetWgs) / std::max(1LL, p.units))});
   return p;
 }
 

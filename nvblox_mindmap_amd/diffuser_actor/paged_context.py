@@ -184,9 +184,9 @@ def append_context(context: ContextPages, k: torch.Tensor, v: torch.Tensor, offs
         raise ValueError("rotary_dim without positions")
     if n == 0 or b == 0 or slots == 0:
         return
-    if k.stride(1) != 1:
+    if k.stride(1) != 1 or k.stride(0) >= 1 << 23:
         k = k.contiguous()
-    if v.stride(1) != 1:
+    if v.stride(1) != 1 or v.stride(0) >= 1 << 23:
         v = v.contiguous()
     _launch(index, _lib.lib().mmf_paged_append, "mmf_paged_append", k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), _TYPES[k.dtype], n, at, axes,
             rotary, rotary_base, offsets.data_ptr(), starts.data_ptr(), table.data_ptr(), b, slots, p, h, hd, n_pages, _TYPES[keys.dtype], keys.data_ptr(),

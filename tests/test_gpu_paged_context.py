@@ -34,6 +34,11 @@ APPEND = [
     (4, 24, 32, [0, 0, 0], [0, 0, 0], 3, "row"),
     (12, 32, 64, list(range(70)), [(7 * i) % 5 for i in range(70)], 4, 32),
     (4, 33, 32, [30], [40], 1, None),
+    (8, 131, 16, [3], [21], 1, None),
+    (8, 255, 32, [0, 40], [33, 9], 1, 254),
+    (16, 64, 128, [7], [300], 1, "row"),
+    (8, 20, 64, [0], [129], 2, 16),
+    (6, 128, 256, [0, 200], [500, 100], 3, "row"),
 ]
 
 
