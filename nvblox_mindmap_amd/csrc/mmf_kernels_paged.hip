@@ -398,7 +398,7 @@ __device__ __forceinline__ Unit unit_of(const AttArgs& a, int unit) {
     u.t = x % a.T;
     u.b = x / a.T;
     u.sel = a.selected + (((long long)u.b * a.T + u.t) * a.H + u.h) * a.count;
-    u.n = a.lengths[u.b] > 0 ? a.count << a.pshift : 0;
+    u.n = a.count << a.pshift;  // (whatever the length: an empty context's keys are masked)
   } else {
     u.t = 0;
     u.b = x;
@@ -848,34 +848,45 @@ __global__ __launch_bounds__(256) void k_paged_score(SelectArgs a) {
   const int unit = blockIdx.x / a.score_blocks, block = blockIdx.x % a.score_blocks;
   const int h = unit % a.H, b = unit / a.H;
   const int P = 1 << a.pshift;
-  const int np = (int)min((long long)a.slots, ((long long)max(a.lengths[b], 0) + P - 1) >> a.pshift);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lc = lane % L, c0 = lc * 8, gp = lane / L;
   const int per_block = 4 * STEP * a.score_steps;
   const int rows = a.T * a.G;
-  if (block * per_block >= np) return;
+  // what does not depend on the context's length is asked for together with it: the first step's table entries, the query
+  auto entries = [&](int first, int (&page)[NP]) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) page[i] = a.table[(long long)b * a.slots + min(first + i * GP + gp, a.slots - 1)];
+  };
+  constexpr int PER = kQueryRows * 8 * L / 256 > 0 ? kQueryRows * 8 * L / 256 : 1;
+  float q0[PER];
   auto query = [&](int r0) {
-    const int n = min(kQueryRows, rows - r0) * 8 * L;
-    for (int i = threadIdx.x; i < n; i += 256) {
-      const int r = r0 + i / (8 * L), c = i % (8 * L);
-      float x = 0.0f;
-      if (c < a.hd) x = to_f(((const T*)a.q)[(((long long)b * a.T + r / a.G) * a.heads + (long long)h * a.G + r % a.G) * a.hd + c]);
-      s_q[i / (8 * L)][c % 8][c / 8] = double2{(double)(x < 0.0f ? 0.0f : x), (double)(x < 0.0f ? x : 0.0f)};  // (a NaN stays)
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int at = threadIdx.x + 256 * i, r = r0 + at / (8 * L), c = at % (8 * L);
+      q0[i] = r < rows && c < a.hd ? to_f(((const T*)a.q)[(((long long)b * a.T + r / a.G) * a.heads + (long long)h * a.G + r % a.G) * a.hd + c]) : 0.0f;
     }
   };
+  auto lay = [&]() {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int at = threadIdx.x + 256 * i, c = at % (8 * L);
+      const float x = q0[i];
+      if (at < kQueryRows * 8 * L) s_q[at / (8 * L)][c % 8][c / 8] = double2{(double)(x < 0.0f ? 0.0f : x), (double)(x < 0.0f ? x : 0.0f)};  // (a NaN stays)
+    }
+  };
+  int page[NP], next[NP];
+  entries(block * per_block + wave * STEP, next);
   query(0);
+  const int np = (int)min((long long)a.slots, ((long long)max(a.lengths[b], 0) + P - 1) >> a.pshift);
+  if (block * per_block >= np) return;
+  lay();
   __syncthreads();
 #pragma unroll 1
   for (int step = 0; step < a.score_steps; ++step) {
     const int first = block * per_block + (step * 4 + wave) * STEP;
     if (rows <= kQueryRows && first >= np) break;  // (with more rows the workgroup stays together: it loads them again)
     double mx[NP][8], mn[NP][8];
-    int page[NP];
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int slot = first + i * GP + gp;
-      page[i] = a.table[(long long)b * a.slots + min(slot, np - 1)];
-      if (page[i] >= a.num_pages || slot >= np) page[i] = -1;
-    }
+    for (int i = 0; i < NP; ++i) page[i] = first + i * GP + gp < np && next[i] < a.num_pages ? next[i] : -1;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const long long at = ((long long)max(page[i], 0) * a.H + h) * W + (W == 96 ? min(c0, 88) : c0);
@@ -890,6 +901,7 @@ __global__ __launch_bounds__(256) void k_paged_score(SelectArgs a) {
         }
       }
     }
+    if (step + 1 < a.score_steps) entries(first + 4 * STEP, next);
     double best[NP];
 #pragma unroll
     for (int i = 0; i < NP; ++i) best[i] = -INFINITY;
@@ -897,8 +909,9 @@ __global__ __launch_bounds__(256) void k_paged_score(SelectArgs a) {
 #pragma unroll 1
     for (int r = 0; r < rows; ++r) {
       if (rows > kQueryRows && r % kQueryRows == 0) {
-        __syncthreads();
         query(r);
+        __syncthreads();
+        lay();
         __syncthreads();
       }
       double s[NP];
@@ -1004,12 +1017,12 @@ __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
   }
   // The bucket of a score, -1: not there.  (Where the step is infinite or no number -- no two finite scores -- all of them are in bucket 0.)
   const float inv = (float)(kBuckets - 1) / (fhi - flo);
-  auto bucket = [&](float x) {
-    if (x == -INFINITY) return -1;
-    if (x != x) return kBuckets - 1;
-    const float y = (x - flo) * inv;
-    return y >= (float)(kBuckets - 1) ? kBuckets - 1 : y > 0.0f ? (int)y : 0;
+  auto bucket = [&](float x) {  // (branch-free: a row of 31 251 spends its time on these instructions)
+    int at = (int)fminf(fmaxf((x - flo) * inv, 0.0f), (float)(kBuckets - 1));
+    at = x != x ? kBuckets - 1 : at;
+    return x == -INFINITY ? -1 : at;
   };
+#pragma unroll 4
   for (int i = tid; i < kept; i += 1024) {
     const int at = bucket(__int_as_float(s_bucket[i]));
     s_bucket[i] = at;
@@ -1144,17 +1157,20 @@ __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
   }
 
   // a wave takes a run of slots: counted, then written behind the waves before it
-  auto taken = [&](int slot) {
-    if (slot >= np) return false;
-    const int at = slot < kept ? s_bucket[slot] : bucket(rounded(sc[slot]));
-    if (at != border) return at > border;
-    if (at < 0) return false;
-    const unsigned long long k = score_key(sc[slot]);
-    return k > last_key || (k == last_key && slot <= last_slot);
+  auto taken = [&](int slot, int end) {
+    const int at = slot < kept ? s_bucket[min(slot, kept - 1)] : slot < end ? bucket(rounded(sc[slot])) : -1;
+    bool take = at > border && slot < end;
+    if (__any(at == border && border >= 0)) {
+      const bool tie = at == border && slot < end;
+      const unsigned long long k = tie ? score_key(sc[slot]) : 0;
+      take = take || (tie && (k > last_key || (k == last_key && slot <= last_slot)));
+    }
+    return __ballot(take);
   };
   const int run = ((np + 15) / 16 + 63) & ~63, from = wave * run, to = min(np, from + run);
   int mine = 0;
-  for (int i = from; i < to; i += 64) mine += __popcll(__ballot(taken(i + lane) && i + lane < to));
+#pragma unroll 4
+  for (int i = from; i < to; i += 64) mine += __popcll(taken(i + lane, to));
   __syncthreads();  // (s_sum's last readers)
   if (lane == 0) s_sum[wave] = mine;
   __syncthreads();
@@ -1164,12 +1180,14 @@ __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
     before += w < wave ? s_sum[w] : 0;
     base += s_sum[w];
   }
-  for (int i = from; i < to; i += 64) {
-    const bool take = taken(i + lane) && i + lane < to;
-    const unsigned long long m = __ballot(take);
-    const int at = before + __popcll(m & ((1ull << lane) - 1));
-    if (take && at < a.count) out[at] = i + lane;
-    before += __popcll(m);
+  if (mine > 0) {
+#pragma unroll 4
+    for (int i = from; i < to; i += 64) {
+      const unsigned long long m = taken(i + lane, to);
+      const int at = before + __popcll(m & ((1ull << lane) - 1));
+      if ((m >> lane & 1) && at < a.count) out[at] = i + lane;
+      before += __popcll(m);
+    }
   }
   for (int i = base + tid; i < a.count; i += 1024) out[i] = -1;
 }
