@@ -9,6 +9,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .paged_context import LayerContext
 from .train_ops import adaln_modulate_train, adaln_usable, add_layer_norm
 from .train_ops import linear as _tlin
 
@@ -126,6 +127,11 @@ class RelativeAttention(nn.Module):
             nn.init.zeros_(lin.bias)
         nn.init.zeros_(self.out_proj.bias)
 
+    def project_paged(self, tokens: torch.Tensor):
+        """(keys, values) of context tokens (n,D) for a paged_context.ContextMemory, which rotates the keys by the tokens' positions."""
+        kv = self.kv_proj(tokens)
+        return kv[:, :self.dim], kv[:, self.dim:]
+
     def project_kv_heads(self, memory: torch.Tensor, kv_rot=None):
         """(head-major keys, transposed values, Lk) of a memory for the matrix-core attention kernel (fused inference;
         AttentionStack consumes 3-tuples in ``kv_caches`` this way)."""
@@ -149,8 +155,16 @@ class RelativeAttention(nn.Module):
     def forward(self, query: torch.Tensor, memory: torch.Tensor, q_rot=None, kv_rot=None,
                 key_padding_mask: Optional[torch.Tensor] = None, need_weights: bool = False, kv_cache=None):
         """query (B,Lq,D), memory (B,Lk,D); key_padding_mask (B,Lk) True = ignore.  Returns (out, weights or None).
-        kv_cache: (keys, values) from project_kv, fused inference path only."""
+        kv_cache: (keys, values) from project_kv, fused inference path only; or a paged_context.LayerContext, whose tokens are
+        attended to in place of `memory` (no autograd, no weights)."""
         B, Lq, D = query.shape
+        if isinstance(kv_cache, LayerContext):
+            if need_weights:
+                raise ValueError("attention weights over a paged context are not formed")
+            q = self.q_proj(query)
+            if q_rot is not None:
+                q = apply_rotary(q, *q_rot)
+            return self.out_proj(kv_cache.attend(q, self.heads)), None
         Lk = memory.shape[1]
         if _fused(query) and not need_weights and (D // self.heads) in (8, 15, 16, 20, 24, 32):  # head dims the kernel is built for
             from .fused_ops import attention_small, rotary_apply
@@ -221,8 +235,11 @@ class AttentionBlock(nn.Module):
             if self.adaln is not None and cond is not None:
                 ss = cond_act.lookup(self.adaln) if isinstance(cond_act, AdaLNBatch) else self.adaln.proj(F.silu(cond) if cond_act is None else cond_act)
             q = FO.q_block(query, ss, A.q_proj, q_rot)
-            k, v = kv_cache if kv_cache is not None else FO.kv_block(memory, A.kv_proj, kv_rot if q_rot is not None else None)
-            att = FO.attention_small(q, k, v, key_padding_mask, A.heads)
+            if isinstance(kv_cache, LayerContext):
+                att = kv_cache.attend(q, A.heads)
+            else:
+                k, v = kv_cache if kv_cache is not None else FO.kv_block(memory, A.kv_proj, kv_rot if q_rot is not None else None)
+                att = FO.attention_small(q, k, v, key_padding_mask, A.heads)
             return FO.attn_out_block(att, query, A.out_proj, self.norm), None
         q_in = self.adaln(query, cond, cond_act) if (self.adaln is not None and cond is not None) else query
         out, w = self.attn(q_in, memory, q_rot, kv_rot, key_padding_mask, need_weights, kv_cache)
@@ -273,7 +290,8 @@ class AttentionStack(nn.Module):
         inference: the attention of a layer and the block kernel behind it run as one launch (fused_ops.cross_layer / self_layer).
         key_padding_mask16: fused_ops.pad_mask16(key_padding_mask) if the caller keeps it (matrix-core attention path).
         cond_act: F.silu(cond), shared by every AdaLN of the pass; kv_caches: per-layer (keys, values) of a memory that
-        is constant across calls (cross-attention at inference)."""
+        is constant across calls (cross-attention at inference), or per-layer paged_context.LayerContext (``ContextMemory.layers``):
+        contexts that grow from call to call; `memory` and the masks are not read then."""
         weights = None
         if (_fused(query) and not need_weights and query.shape[-1] in _block_dims() and len(self.attn) > 0
                 and (query.shape[-1] // self.attn[0].attn.heads) in (8, 15, 16, 20, 24, 32) and self.ffw[0].fc1.out_features == query.shape[-1]):
@@ -318,7 +336,8 @@ class AttentionStack(nn.Module):
             qh_next = None
             for li, (blk, ffw) in enumerate(zip(self.attn, self.ffw)):
                 A = blk.attn
-                if (not self.self_attention and kv_caches is not None and len(kv_caches[li]) == 3
+                paged = kv_caches is not None and isinstance(kv_caches[li], LayerContext)
+                if (not self.self_attention and kv_caches is not None and not paged and len(kv_caches[li]) == 3
                         and (query.shape[-1], A.heads) == FO.MFMA_DIMS):
                     # cross-attention over a context whose head-major keys / values were cached (project_kv_heads): per layer
                     # attention | (out_proj + LN + FFN + the NEXT layer's query projection)
@@ -357,8 +376,9 @@ class AttentionStack(nn.Module):
                     q, k, v = FO.qkv_block(query, ss_of(blk.adaln), A.q_proj, A.kv_proj, q_rot)
                 else:
                     q = FO.q_block(query, ss_of(blk.adaln), A.q_proj, q_rot)
-                    k, v = kv_caches[li] if kv_caches is not None else FO.kv_block(memory, A.kv_proj, kv_rot if q_rot is not None else None)
-                att = FO.attention_small(q, k, v, key_padding_mask, A.heads)
+                    if not paged:
+                        k, v = kv_caches[li] if kv_caches is not None else FO.kv_block(memory, A.kv_proj, kv_rot if q_rot is not None else None)
+                att = kv_caches[li].attend(q, A.heads) if paged and not self.self_attention else FO.attention_small(q, k, v, key_padding_mask, A.heads)
                 query = FO.out_ffn_block(att, query, A.out_proj, blk.norm, ss_of(ffw.adaln), ffw.fc1, ffw.fc2, ffw.norm)
             return query, None
         for li, (attn, ffw) in enumerate(zip(self.attn, self.ffw)):

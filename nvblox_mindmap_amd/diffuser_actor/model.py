@@ -24,6 +24,7 @@ from .fps import farthest_point_sampling, farthest_point_sampling_cpu
 from . import layers as layers_mod
 from .layers import AttentionBlock, AttentionStack, FeedForwardBlock, rotary3d, sinusoidal_embedding
 from .loss import LossWeights, compute_loss
+from .paged_context import ContextMemory
 from .relative_conversions import (get_current_pose_from_gripper_history, to_absolute_trajectory, to_relative_gripper_history,
                                    to_relative_pcd, to_relative_trajectory)
 from .rotations import normalize_pointcloud, normalize_pos, normalize_trajectory, unnormalize_trajectory
@@ -210,15 +211,20 @@ class DiffusionHead(nn.Module):
              "ctx_rot": rotary3d(enc["context_pos"], D), "fps_rot": rotary3d(enc["fps_pos"], D),
              "history": self.history_mlp(enc["history_feats"].flatten(1)), "cross_kv": None}
         P["adaln"] = None
+        memory = enc.get("context_memory")
+        if memory is not None:  # the cross-attention reads the memory's pages in place of this observation's context
+            P["cross_kv"] = [layer for layer in memory.layers]
         if layers_mod._fused(ctx_feats):  # keys / values of the (step-invariant) context, once per inference instead of per step
-            P["cross_kv"] = [blk.attn.project_kv(ctx_feats, P["ctx_rot"]) for blk in self.cross_attn.attn]
+            if memory is None:
+                P["cross_kv"] = [blk.attn.project_kv(ctx_feats, P["ctx_rot"]) for blk in self.cross_attn.attn]
             P["adaln"] = layers_mod.AdaLNBatch([mod for mod in self.modules() if isinstance(mod, layers_mod.AdaLN)])
             from .fused_ops import MFMA_DIMS
 
             if (D, self.cfg.num_attn_heads) == MFMA_DIMS:
                 from .fused_ops import pad_mask16
 
-                P["cross_kv"] = [blk.attn.project_kv_heads(ctx_feats, P["ctx_rot"]) for blk in self.cross_attn.attn]
+                if memory is None:
+                    P["cross_kv"] = [blk.attn.project_kv_heads(ctx_feats, P["ctx_rot"]) for blk in self.cross_attn.attn]
                 P["ctx_pad16"] = pad_mask16(P["ctx_pad"])
                 from .fused_ops import CrossHandover
 
@@ -247,6 +253,18 @@ class DiffusionHead(nn.Module):
                 P["rot_freq"] = torch.exp(torch.arange(0, third, 2, device=dev, dtype=torch.float32) * (-math.log(10000.0) / third))
         return P
 
+    @torch.no_grad()
+    def extend_memory(self, memory, enc):
+        """Append an observation's valid context tokens to a paged_context.ContextMemory (one context per sample): the keys and values
+        of the cross-attention layers, rotated by the tokens' positions.  Synchronises (the tokens are counted on the host)."""
+        mask = enc["context_mask"]
+        if mask.shape[0] != memory.contexts or len(memory.layers) != len(self.cross_attn.attn):
+            raise ValueError(f"a memory of {memory.contexts} contexts and {len(memory.layers)} layers for {mask.shape[0]} samples and "
+                             f"{len(self.cross_attn.attn)} cross-attention layers")
+        counts = mask.sum(dim=1).tolist()
+        tokens, positions = enc["context_feats"][mask], enc["context_pos"][mask].to(torch.float32).contiguous()
+        memory.append(counts, [blk.attn.project_paged(tokens) for blk in self.cross_attn.attn], positions, self.cfg.embedding_dim)
+
     def time_embeddings(self, timesteps, device):
         """time_mlp(sinusoidal(t)) for a list of timesteps in one batched pass ([T, D]): the time part of the conditioning
         vector depends on the step only, not on the inputs."""
@@ -265,6 +283,8 @@ class DiffusionHead(nn.Module):
         B, L, G, _ = trajectory.shape
         nt = L * G
         P = prepared if prepared is not None else self.prepare_context(enc)
+        if need_weights and P["cross_kv"] is not None and enc.get("context_memory") is not None:
+            raise ValueError("attention weights over a context memory are not formed")
         if (not need_weights and time_emb is not None and P.get("seq") is not None and layers_mod._fused(trajectory)
                 and nt == P["pos_table"].shape[0] and G <= 4 and not cfg.use_instruction):
             return self._forward_fused(trajectory, P, time_emb)
@@ -478,7 +498,8 @@ class DiffuserActor(nn.Module):
         self._inference_timesteps = self.position_noise_scheduler.timesteps.tolist()
         shape = (1 + len(self._inference_timesteps), batch, cfg.prediction_horizon, cfg.ngrippers, 9)
         noise = torch.randn(shape, device=device, generator=generator)
-        if self._graph_sampler is not None and torch.device(device).type == "cuda" and not torch.is_grad_enabled():
+        # (a context memory's pages are not among the graph's static inputs: its loop runs eagerly)
+        if self._graph_sampler is not None and torch.device(device).type == "cuda" and not torch.is_grad_enabled() and enc.get("context_memory") is None:
             return self._graph_sampler.run(enc, noise)
         return self._denoise(enc, noise)
 
@@ -487,6 +508,15 @@ class DiffuserActor(nn.Module):
         """Use the fused HIP ops (rotary, AdaLN, small attention; cached context keys/values) in blocks that run without
         autograd on the GPU.  Process-wide switch; training (autograd on) always takes the composite torch ops."""
         layers_mod.FUSED_INFERENCE = bool(on)
+
+    def new_context_memory(self, contexts: int, num_pages: int, page_size: int = 64, dtype: torch.dtype = torch.float32, slots: Optional[int] = None,
+                           selected_pages: Optional[int] = None, device="cuda") -> ContextMemory:
+        """Pages for what the cross-attention keeps of earlier observations (``forward(..., context_memory=)``): ``contexts`` robots,
+        ``num_pages`` pages of ``page_size`` tokens in each layer's pool, at most ``slots`` of them per robot.  ``selected_pages``: attend through
+        the best so many pages of a context (paged_context.select_pages) instead of all."""
+        cfg = self.cfg
+        return ContextMemory(len(self.prediction_head.cross_attn.attn), contexts, num_pages, cfg.num_attn_heads, cfg.embedding_dim // cfg.num_attn_heads,
+                             page_size, dtype, slots, selected_pages, device)
 
     def enable_graph_sampling(self, on: bool = True) -> None:
         """Replay the denoising loop (T steps x ~150 small kernels, launch-bound at batch 1) as a captured HIP graph.
@@ -498,15 +528,24 @@ class DiffuserActor(nn.Module):
 
     # -- forward --------------------------------------------------------------------------------------------------------
     def forward(self, gt_gripper_pred, gt_head_yaw, rgb_obs, pcd_obs, pcd_valid_mask, vertex_features, vertices,
-                vertices_valid_mask, instruction, gripper_history, run_inference: bool = False, backbone_feats=None):
+                vertices_valid_mask, instruction, gripper_history, run_inference: bool = False, backbone_feats=None,
+                context_memory: Optional[ContextMemory] = None):
         """Arguments as in the reference (diffuser_actor.py:518-531):
           gt_gripper_pred (B,L,ngrip,8) xyz + quaternion + openness (or None at inference), gt_head_yaw (B,L,1),
           rgb_obs (B,ncam,3,H,W) in [0,1], pcd_obs (B,ncam,3,H,W) world points, pcd_valid_mask (B,ncam,H,W),
           vertex_features (B,N,C), vertices (B,N,3) world, vertices_valid_mask (B,N), instruction (B,T,512) or None,
           gripper_history (B,nhist,ngrip,8).
         Training: returns ((total, pos, rot, gripper, head_yaw) losses, encoded inputs, None).
-        Inference: returns (trajectory (B,L,ngrip,8), head_yaw, losses or None, encoded inputs, None)."""
+        Inference: returns (trajectory (B,L,ngrip,8), head_yaw, losses or None, encoded inputs, None).
+        context_memory (inference, ``new_context_memory``): this observation's valid context tokens are appended to it, and the trajectory
+        attends to all that it holds -- every observation since the context was released -- instead of this observation's context
+        alone; the gripper history and the sub-sampled context stay this observation's."""
         cfg, wb = self.cfg, self.workspace_bounds
+        if context_memory is not None:
+            if not run_inference or torch.is_grad_enabled():
+                raise ValueError("context_memory: inference under torch.no_grad() only")
+            if cfg.relative_action:
+                raise ValueError("context_memory: with relative_action every observation has a frame of its own")
         closedness = gripper_history[..., 7:8]
         history = gripper_history[..., :7]
         current_pose = None
@@ -535,6 +574,9 @@ class DiffuserActor(nn.Module):
                                      instruction, history, closedness, backbone_feats)
         B, dev = history.shape[0], history.device
         if run_inference:
+            if context_memory is not None:
+                self.prediction_head.extend_memory(context_memory, enc)
+                enc["context_memory"] = context_memory
             traj, head_yaw = self.sample_trajectory(enc, B, dev)
             losses = None
             if gt is not None:

@@ -8,9 +8,10 @@ is not projected again, and a long context can be attended to through its few re
 
 ``ContextPages`` names the buffers of one layer, ``append_context`` / ``context_attention`` / ``select_pages`` are the operators over
 them (float32, float16, bfloat16; no autograd; nothing synchronises, all lengths are read on the device, so calls can be captured into
-a graph and replayed with other lengths)."""
+a graph and replayed with other lengths).  ``PageTable`` hands out a pool's pages to contexts, ``ContextMemory`` puts the table and the
+pages of a stack's layers together: what ``DiffuserActor`` keeps of earlier observations (``new_context_memory``)."""
 import functools
-from typing import NamedTuple, Optional
+from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -267,3 +268,125 @@ def select_pages(q: torch.Tensor, context: ContextPages, table: torch.Tensor, le
     _launch(index, _lib.lib().mmf_paged_select, "mmf_paged_select", q.data_ptr(), context.key_min.data_ptr(), context.key_max.data_ptr(), _TYPES[q.dtype],
             table.data_ptr(), lengths.data_ptr(), b, t, h, heads // h, hd, slots, n_pages, p, count, out.data_ptr(), work.data_ptr(), need)
     return out
+
+
+class PageTable:
+    """Which pages of a pool belong to which context: the bookkeeping on the host, ``table`` [contexts, slots] and ``lengths`` [contexts] int32
+    on the device, changed in place (a captured graph reads the new ones).  A page belongs to one context."""
+
+    def __init__(self, contexts: int, num_pages: int, page_size: int, slots: Optional[int] = None, device="cuda"):
+        if contexts < 1 or num_pages < 1 or page_size not in PAGE_SIZES:
+            raise ValueError(f"positive sizes, page_size one of {PAGE_SIZES}")
+        self.page_size, self.num_pages = page_size, num_pages
+        self.slots = num_pages if slots is None else int(slots)
+        if self.slots < 1:
+            raise ValueError("slots has to be positive")
+        self._free = list(range(num_pages - 1, -1, -1))
+        self._pages: List[List[int]] = [[] for _ in range(contexts)]
+        self._held = [0] * contexts
+        self.table = torch.full((contexts, self.slots), -1, dtype=torch.int32, device=device)
+        self.lengths = torch.zeros(contexts, dtype=torch.int32, device=device)
+
+    @property
+    def held(self) -> Tuple[int, ...]:
+        """Tokens of each context (on the host)."""
+        return tuple(self._held)
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def _needed(self, counts: Sequence[int]) -> List[int]:
+        if len(counts) != len(self._held) or any(int(c) < 0 for c in counts):
+            raise ValueError(f"{len(self._held)} counts of zero or more tokens: got {list(counts)}")
+        return [-(-(h + int(c)) // self.page_size) for h, c in zip(self._held, counts)]
+
+    def check(self, counts: Sequence[int]) -> None:
+        """Raise unless every context can take that many tokens more."""
+        need = self._needed(counts)
+        over = [b for b, n in enumerate(need) if n > self.slots]
+        if over:
+            raise RuntimeError(f"contexts {over} would pass {self.slots} pages of {self.page_size} tokens")
+        wanted = sum(n - len(p) for n, p in zip(need, self._pages))
+        if wanted > len(self._free):
+            raise RuntimeError(f"{wanted} pages wanted, {len(self._free)} of {self.num_pages} free: release a context or make the pool larger")
+
+    def extend(self, counts: Sequence[int]) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Pages for ``counts[b]`` tokens more of every context.  -> (offsets [contexts + 1], starts [contexts]) of ``append_context``;
+        ``lengths`` counts the new tokens from here on.  Raises, and changes nothing, where the pool or a context's slots do not suffice."""
+        self.check(counts)
+        device = self.table.device
+        starts = torch.tensor(self._held, dtype=torch.int32).to(device)
+        offsets = [0]
+        rows, cols, ids = [], [], []
+        for b, (need, c) in enumerate(zip(self._needed(counts), counts)):
+            while len(self._pages[b]) < need:
+                page = self._free.pop()
+                rows.append(b), cols.append(len(self._pages[b])), ids.append(page)
+                self._pages[b].append(page)
+            self._held[b] += int(c)
+            offsets.append(offsets[-1] + int(c))
+        if ids:
+            self.table[torch.tensor(rows, device=device), torch.tensor(cols, device=device)] = torch.tensor(ids, dtype=torch.int32, device=device)
+        self.lengths.copy_(torch.tensor(self._held, dtype=torch.int32))
+        return torch.tensor(offsets, dtype=torch.int32).to(device), starts
+
+    def release(self, context: int) -> None:
+        """Forget a context; its pages go back to the pool."""
+        self._free.extend(reversed(self._pages[context]))
+        self._pages[context] = []
+        self._held[context] = 0
+        self.table[context].fill_(-1)
+        self.lengths[context].zero_()
+
+
+class LayerContext:
+    """One layer's share of a ``ContextMemory``: what an attention layer takes in place of cached keys and values."""
+
+    def __init__(self, memory: "ContextMemory", pages: ContextPages):
+        self.memory, self.pages = memory, pages
+
+    def attend(self, q: torch.Tensor, heads: int) -> torch.Tensor:
+        """softmax(q k^T / sqrt(head_dim)) v of rotated queries [contexts, T, heads * head_dim] over the memory (over its
+        ``selected_pages`` best pages where that is set); 16-bit pages: q is rounded to their type, the result is of q's."""
+        m, t = self.memory, self.memory.pages_of
+        x = q if q.dtype is self.pages.keys.dtype else q.to(self.pages.keys.dtype)
+        chosen = None if m.selected_pages is None else select_pages(x, self.pages, t.table, t.lengths, heads, m.selected_pages)
+        return context_attention(x, self.pages, t.table, t.lengths, heads, pages=chosen).to(q.dtype)
+
+
+class ContextMemory:
+    """Growing contexts of the attention layers of a stack: one page table, one set of pages per layer.  ``layers[i]`` is layer i's
+    ``LayerContext``."""
+
+    def __init__(self, layers: int, contexts: int, num_pages: int, kv_heads: int, head_dim: int, page_size: int = 64,
+                 dtype: torch.dtype = torch.float32, slots: Optional[int] = None, selected_pages: Optional[int] = None, device="cuda"):
+        if layers < 1 or (selected_pages is not None and selected_pages < 1):
+            raise ValueError("layers and selected_pages have to be positive")
+        self.pages_of = PageTable(contexts, num_pages, page_size, slots, device)
+        self.selected_pages = selected_pages
+        self.layers = [LayerContext(self, allocate_pages(num_pages, kv_heads, head_dim, page_size, dtype, device)) for _ in range(layers)]
+
+    @property
+    def contexts(self) -> int:
+        return self.pages_of.table.shape[0]
+
+    @property
+    def held(self) -> Tuple[int, ...]:
+        return self.pages_of.held
+
+    def append(self, counts: Sequence[int], keys_values: Sequence[Tuple[torch.Tensor, torch.Tensor]], positions: Optional[torch.Tensor] = None,
+               rotary_dim: Optional[int] = None) -> None:
+        """``counts[b]`` tokens more of every context: their (keys, values) of each layer, rows in the contexts' order, and positions."""
+        if len(keys_values) != len(self.layers):
+            raise ValueError(f"{len(self.layers)} layers' keys and values: got {len(keys_values)}")
+        n = sum(int(c) for c in counts)
+        for k, v in keys_values:
+            if k.dim() != 2 or k.shape[0] != n or v.shape != k.shape:
+                raise ValueError(f"keys and values of {n} tokens: got {tuple(k.shape)}, {tuple(v.shape)}")
+        offsets, starts = self.pages_of.extend(counts)
+        for layer, (k, v) in zip(self.layers, keys_values):
+            append_context(layer.pages, k, v, offsets, starts, self.pages_of.table, positions, rotary_dim)
+
+    def release(self, context: int) -> None:
+        self.pages_of.release(context)

@@ -111,3 +111,60 @@ def test_workspace_sizes():
     assert L.mmf_paged_attention_workspace_bytes(1, 1, 1, 1, 16, 100, 0) == 0  # one split: no partial results
     assert L.mmf_paged_attention_workspace_bytes(1, 1, 8, 4, 128, 1 << 20, 0) > 0
     assert L.mmf_paged_attention_workspace_bytes(0, 1, 8, 4, 128, 1 << 20, 0) == 0
+
+
+# ---- the page table -------------------------------------------------------------------------------------------------------------------
+def test_page_table_hands_out_each_page_once():
+    t = P.PageTable(3, 10, 16, slots=6, device="cpu")
+    offsets, starts = t.extend([17, 0, 16])
+    assert offsets.tolist() == [0, 17, 17, 33] and starts.tolist() == [0, 0, 0] and offsets.dtype == starts.dtype == torch.int32
+    assert t.held == (17, 0, 16) and t.lengths.tolist() == [17, 0, 16] and t.free_pages == 7
+    offsets, starts = t.extend([15, 1, 1])  # context 0 fills its second page
+    assert starts.tolist() == [17, 0, 16] and t.free_pages == 5
+    used = [p for p in t.table.flatten().tolist() if p >= 0]
+    assert sorted(used) == sorted(set(used)) and len(used) == 5 and (t.table[0] >= 0).sum() == 2
+    before = (t.table.clone(), t.held, t.free_pages)
+    with pytest.raises(RuntimeError, match="free"):
+        t.extend([0, 80, 16])
+    with pytest.raises(RuntimeError, match="would pass"):
+        t.extend([65, 0, 0])
+    for bad in ([1, 2], [1, -1, 0]):
+        with pytest.raises(ValueError):
+            t.extend(bad)
+    assert torch.equal(t.table, before[0]) and t.held == before[1] and t.free_pages == before[2]
+    t.release(0)
+    assert t.free_pages == 7 and t.held == (0, 1, 17) and t.table[0].tolist() == [-1] * 6 and t.lengths.tolist() == [0, 1, 17]
+    t.extend([96, 0, 0])
+    used = [p for p in t.table.flatten().tolist() if p >= 0]
+    assert len(used) == len(set(used)) == 9
+
+
+def test_memory_is_checked():
+    with pytest.raises(ValueError):
+        P.ContextMemory(0, 1, 4, 2, 16, 16, device="cpu")
+    with pytest.raises(ValueError):
+        P.ContextMemory(1, 1, 4, 2, 16, 16, selected_pages=0, device="cpu")
+    with pytest.raises(ValueError):
+        P.PageTable(1, 4, 17, device="cpu")
+    m = P.ContextMemory(2, 2, 4, 2, 16, 16, device="cpu")
+    k = torch.zeros(3, 32)
+    with pytest.raises(ValueError, match="2 layers"):
+        m.append([1, 2], [(k, k)])
+    with pytest.raises(ValueError, match="of 4 tokens"):
+        m.append([1, 3], [(k, k), (k, k)])
+    assert m.held == (0, 0)
+
+
+def test_model_refuses_a_memory_where_it_has_no_meaning():
+    from nvblox_mindmap_amd.diffuser_actor import DiffuserActor, DiffuserActorConfig
+
+    cfg = DiffuserActorConfig(data_type="mesh", feature_dim=8, relative_action=True)
+    model = DiffuserActor(cfg, torch.tensor([[-1.0, -1, -1], [1, 1, 1]]))
+    memory = model.new_context_memory(1, 4, 16, device="cpu")
+    assert len(memory.layers) == 2 and memory.layers[0].pages.head_dim == 15
+    args = [None] * 10
+    args[9] = torch.zeros(1, 3, 2, 8)
+    with pytest.raises(ValueError, match="inference"):
+        model(*args, context_memory=memory)
+    with torch.no_grad(), pytest.raises(ValueError, match="relative_action"):
+        model(*args, run_inference=True, context_memory=memory)
