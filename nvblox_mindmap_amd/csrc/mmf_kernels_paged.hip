@@ -32,11 +32,6 @@ struct alignas(sizeof(T) * N) Pack {
   T v[N];
 };
 
-template <class T, int N>
-struct __attribute__((packed, aligned(sizeof(T)))) Loose {  // the same, aligned like one element
-  T v[N];
-};
-
 template <class T>
 __device__ __forceinline__ float to_f(T x) {
   return (float)x;
@@ -130,14 +125,19 @@ __device__ __forceinline__ bool find_segment(const AppendArgs& a, int unit, Segm
 // that may belong to two heads, whose rotation pairs are still the lane's own (the policy's heads of 15); 0: any layout, one channel,
 // its partner read beside it.  The page is taken in blocks of tokens whose cos / sin fit into LDS: computed once for all heads (of the row's
 // own pairs where the code covers the whole row), at [slot of a group][chunk of pairs][group], the order in which lanes read them.
-constexpr int kAppendRow = 1024;  // channels of a workgroup at most
+// KIND 1 puts the block's keys together in LDS and stores them from there in 16-byte pieces of the pages, padding included (stored
+// as the lanes have them, 4 + 12 bytes or 4 times 4, the keys took 11 us of 43 for 32 contexts of 8 heads of 15).
+template <int KIND>
+constexpr int kAppendRow = KIND == 1 ? 256 : 1024;  // channels of a workgroup at most
 template <class TI, class T, int KIND>
 __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
   constexpr int VT = 16 / sizeof(T), VEC = KIND ? VT : 1, NP = VEC > 1 ? VEC / 2 : 1;
   constexpr int kAngles = sizeof(T) == 4 ? 2048 : 4096;  // (the 32-bit kernels have the registers for more workgroups a CU than 32 KB leave room for)
   __shared__ __attribute__((aligned(16))) float2 s_angle[kAngles];
-  __shared__ double s_turns[kAppendRow / 2 + 8];    // turns a unit of position, by pair
-  __shared__ float s_lo[kAppendRow], s_hi[kAppendRow];
+  constexpr int ROW = kAppendRow<KIND>, kTile = KIND == 1 ? 4096 * 4 / sizeof(T) : 0;
+  __shared__ double s_turns[ROW / 2 + 8];           // turns a unit of position, by pair
+  __shared__ float s_lo[ROW], s_hi[ROW];
+  __shared__ __attribute__((aligned(16))) T s_tile[KIND == 1 ? kTile : 1];  // [slot of the block][channel of the workgroup]
   Segment seg;
   if (!find_segment(a, blockIdx.x, seg)) return;
   const int page = a.table[(long long)seg.b * a.slots + seg.slot];
@@ -160,9 +160,11 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
     s_turns[i] = exp2(-a.log2_base * (double)j / (double)span) * 0.15915494309189533576888;
   }
   const int pair_chunks = (pairs + NP - 1) / NP;
-  const int groups = pairs ? min(256 / VT, kAngles / (pair_chunks * NP * VT)) : 256 / VT, block = groups * VT;  // of a block
+  int groups = pairs ? min(256 / VT, kAngles / (pair_chunks * NP * VT)) : 256 / VT;  // of a block
+  if (KIND == 1) groups = min(groups, kTile / (nh * a.hd * VT));
+  const int block = groups * VT;
   // what the page's summary held (it begins anew with its first slot), asked for early: the first access to a page of a large pool waits long
-  constexpr int OLD = kAppendRow / 256;
+  constexpr int OLD = ROW / 256;
   const bool merge = seg.first > 0;
   float old_lo[OLD], old_hi[OLD];
   if (merge) {
@@ -198,14 +200,13 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
     for (int ch = tid / gw; ch < nchunks; ch += 256 / gw) {
       const int c = c0 + ch * VEC;  // channel in the row
       const int h = c / a.hd, d = c - h * a.hd;
-      const bool one_head = KIND != 1 || d + VEC <= a.hd;
-      unsigned kat[VEC], vat[VEC];  // where slot 0 of channel c + i is in the page's keys and values
+      unsigned kat[1], vat[VEC];  // where slot 0 of channel c (c + i) is in the page's keys (values)
       int pair[NP];                 // its pair in the table, or -1
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         const int over = KIND == 1 && d + i >= a.hd ? (d + i) / a.hd : 0;
         const int hh = h + over, dd = d + i - over * a.hd;
-        kat[i] = ((unsigned)hh << a.pshift) * a.W + dd;
+        if (i == 0) kat[0] = ((unsigned)hh << a.pshift) * a.W + dd;
         vat[i] = ((unsigned)hh * a.W + dd) << a.pshift;
         if (i % 2 == 0) {
           const int w = whole_row ? c + i : dd;
@@ -273,14 +274,8 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
 #pragma unroll
           for (int t = 0; t < VT; ++t) {
             T* to = kpage + ((unsigned)(slot0 + t) * a.W + kat[0]);
-            if (KIND == 2) {
-              *reinterpret_cast<Pack<T, VEC>*>(to) = out[t];
-            } else if (one_head) {
-              *reinterpret_cast<Loose<T, VEC>*>(to) = __builtin_bit_cast(Loose<T, VEC>, out[t]);  // (16 bytes, aligned like the type)
-            } else {
-#pragma unroll
-              for (int i = 0; i < VEC; ++i) kpage[(unsigned)(slot0 + t) * a.W + kat[i]] = out[t].v[i];
-            }
+            if (KIND == 1) to = s_tile + (slot0 + t - first) * (nh * a.hd) + ch * VEC;
+            *reinterpret_cast<Pack<T, VEC>*>(to) = out[t];
           }
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
@@ -293,12 +288,11 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
 #pragma unroll
           for (int t = 0; t < VT; ++t)
             if (slot0 + t >= lo_slot && slot0 + t < hi_slot) {
-              if (KIND == 2) *reinterpret_cast<Pack<T, VEC>*>(kpage + ((unsigned)(slot0 + t) * a.W + kat[0])) = out[t];
+              T* to = kpage + ((unsigned)(slot0 + t) * a.W + kat[0]);
+              if (KIND == 1) to = s_tile + (slot0 + t - first) * (nh * a.hd) + ch * VEC;
+              *reinterpret_cast<Pack<T, VEC>*>(to) = out[t];
 #pragma unroll
-              for (int i = 0; i < VEC; ++i) {
-                if (KIND != 2) kpage[(unsigned)(slot0 + t) * a.W + kat[i]] = out[t].v[i];
-                vpage[vat[i] + (unsigned)(slot0 + t)] = (T)to_f(vr[t].v[i]);
-              }
+              for (int i = 0; i < VEC; ++i) vpage[vat[i] + (unsigned)(slot0 + t)] = (T)to_f(vr[t].v[i]);
             }
         }
       }
@@ -321,6 +315,18 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
     }
     begun = true;
     __syncthreads();
+    if constexpr (KIND == 1) {
+      const int wide = (a.hd + VEC - 1) / VEC, each = nh * wide;  // 16-byte pieces of a head, of a slot
+      for (int i = tid; i < (hi_slot - lo_slot) * each; i += 256) {
+        const int s = i / each, h = (i - s * each) / wide, d = (i - s * each - h * wide) * VEC;
+        const T* from = s_tile + (lo_slot + s - first) * (nh * a.hd) + h * a.hd + d;
+        Pack<T, VEC> out;
+#pragma unroll
+        for (int x = 0; x < VEC; ++x) out.v[x] = d + x < a.hd ? from[min(x, a.hd - 1 - d)] : (T)0.0f;
+        *reinterpret_cast<Pack<T, VEC>*>(kpage + (((unsigned)(h0 + h) << a.pshift) * a.W + (unsigned)(lo_slot + s) * a.W + d)) = out;
+      }
+      __syncthreads();
+    }
   }
 #pragma unroll
   for (int j = 0; j < OLD; ++j) {
@@ -1197,18 +1203,22 @@ void append_typed(AppendArgs& a, int units, hipStream_t s) {
   constexpr int VEC = 16 / sizeof(T);  // 16-byte stores both ways
   // wide loads need whole chunks in a workgroup's heads, every chunk of the row at a multiple of its size, and rotation pairs that start at even channels of the row
   const uintptr_t align = sizeof(TI) * VEC;
-  const bool wide = VEC / std::gcd(a.hd, VEC) * a.hd <= kAppendRow && (a.H * a.hd) % VEC == 0 && a.k_stride % VEC == 0 && a.v_stride % VEC == 0 && (uintptr_t)a.k % align == 0 && (uintptr_t)a.v % align == 0 &&
+  const bool whole = a.hd % VEC == 0;
+  const int most = whole ? kAppendRow<2> : kAppendRow<1>;
+  const bool wide = VEC / std::gcd(a.hd, VEC) * a.hd <= most && (a.H * a.hd) % VEC == 0 && a.k_stride % VEC == 0 && a.v_stride % VEC == 0 && (uintptr_t)a.k % align == 0 && (uintptr_t)a.v % align == 0 &&
                     (a.rotary == 0 || a.rotary > a.hd || a.hd % 2 == 0);
   // heads of a workgroup: as many workgroups as keep the chip busy, but not fewer than 128 chunks each (of a context's mean number of
-  // tokens); whole chunks, at most kAppendRow channels
+  // tokens); whole chunks, not more channels than its tables hold
   const int step = wide ? VEC : 1, unit = step / std::gcd(a.hd, step);
   const int groups = std::max(1, std::min(a.n_tokens / a.B, 1 << a.pshift) / VEC);
   const long long chunks = (long long)a.H * a.hd / step * groups;
   const int parts = (int)std::max(1LL, std::min<long long>({a.H, 2048 / units, chunks / 128}));
-  a.heads_per_wg = std::min((a.H + parts - 1) / parts, std::max(1, kAppendRow / a.hd));
+  // (a tile of 16 KB: 64 tokens of 64 32-bit channels, 128 of 16 bits)
+  const int channels = wide ? (whole ? most : 64 * VEC / 4) : kAppendRow<0>;
+  a.heads_per_wg = std::min((a.H + parts - 1) / parts, std::max(1, channels / a.hd));
   a.heads_per_wg = std::max(a.heads_per_wg / unit, 1) * unit;
   const dim3 grid(units, (a.H + a.heads_per_wg - 1) / a.heads_per_wg);
-  if (wide && a.hd % VEC == 0) k_paged_append<TI, T, 2><<<grid, 256, 0, s>>>(a);
+  if (wide && whole) k_paged_append<TI, T, 2><<<grid, 256, 0, s>>>(a);
   else if (wide) k_paged_append<TI, T, 1><<<grid, 256, 0, s>>>(a);
   else k_paged_append<TI, T, 0><<<grid, 256, 0, s>>>(a);
 }
