@@ -581,7 +581,7 @@ const char* paged_shape_error(int type, int B, int slots, int page_size, int H, 
   if (B <= 0 || slots <= 0 || H <= 0 || num_pages <= 0) return "positive sizes";
   if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1))) return "page_size is 16, 32, 64, 128 or 256";
   if (paged_width(head_dim) == 0) return "1 <= head_dim <= 256";
-  if ((int64_t)slots * page_size > 0x7fffff00LL) return "slots * page_size passes 31 bits";
+  if ((int64_t)slots * page_size > (1 << 30)) return "slots * page_size passes 2^30";
   if ((int64_t)H * page_size * paged_width(head_dim) > (1 << 30)) return "a page passes 2^30 elements";
   return nullptr;
 }
@@ -610,7 +610,7 @@ int mmf_paged_append(const void* k, int64_t k_row_stride, const void* v, int64_t
   if (launch_paged_append(k, k_row_stride, v, v_row_stride, in_type, (int)tokens, positions, rotary_dim ? axes : 1, rotary_dim, rotary_base, offsets,
                           starts, table, B, slots, page_shift(page_size), kv_heads, head_dim, num_pages, type, keys, values, key_min, key_max,
                           (hipStream_t)stream) != 0)
-    return paged_fail(name, "types");
+    return paged_fail(name, "too many tokens or heads for one call");
   return check_launch();
 }
 
@@ -627,7 +627,7 @@ int mmf_paged_attention(const void* q, const void* keys, const void* values, int
   if (!q || !keys || !values || !table || !lengths || !out) return paged_fail(name, "null pointer");
   if (T <= 0 || group <= 0 || (int64_t)T * group > (1 << 24) || (int64_t)kv_heads * group * head_dim > 0x7fffffffLL)
     return paged_fail(name, "positive T and group");
-  if (selected && (count <= 0 || (int64_t)count * page_size > 0x7fffff00LL)) return paged_fail(name, "count > 0, count * page_size below 2^31");
+  if (selected && (count <= 0 || (int64_t)count * page_size > (1 << 30))) return paged_fail(name, "count > 0, count * page_size up to 2^30");
   const int64_t need = mmf_paged_attention_workspace_bytes(B, T, kv_heads, group, head_dim, (int64_t)(selected ? count : slots) * page_size, selected != nullptr);
   if (workspace_bytes < need || (need > 0 && !workspace)) return paged_fail(name, "workspace smaller than mmf_paged_attention_workspace_bytes");
   const int rc = launch_paged_attention(q, keys, values, type, table, lengths, selected, count, B, T, kv_heads, group, head_dim, slots, num_pages,

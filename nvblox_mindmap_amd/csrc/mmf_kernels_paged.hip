@@ -958,9 +958,11 @@ constexpr unsigned long long kNotThere = 0x000fffffffffffffull;  // score_key(-i
 
 // The count best of a row, the lowest slots first among equals, written in ascending order.  The scores are rounded to 32 bits (a monotone map: they
 // sort into buckets as the scores do) and their buckets kept in LDS (the part of a row behind CAP pages is read again in each pass); the
-// scores themselves are read again only where two of a bucket have to be told apart.  A histogram over 2048 equal steps between the smallest and the largest finds the bucket that holds the border;
-// up to kFew of a bucket are ranked against each other by score and slot.  A bucket with more (many near-equals, or a few scores far
-// from the rest) is divided again by the scores' bits as integers, from their highest differing bit: 11 bits a pass, so it ends.
+// scores themselves are read again only where two of a bucket have to be told apart.  A histogram over 2048 equal steps between the
+// smallest and the largest finds the bucket that holds the border; up to kFew of a bucket are ranked against each other by score and
+// slot.  A bucket with more (many near-equals, or a few scores far from the rest) is divided again by the scores' bits as integers, from
+// their highest differing bit: 11 bits a pass, so it ends.  One workgroup a row: what bounds a long row is what a CU reads and handles (29 us
+// for 31 251 pages; 6 us for 400).
 constexpr int kBuckets = 2048, kFew = 256;
 template <int CAP>
 __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
@@ -1175,7 +1177,6 @@ __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
   };
   const int run = ((np + 15) / 16 + 63) & ~63, from = wave * run, to = min(np, from + run);
   int mine = 0;
-#pragma unroll 4
   for (int i = from; i < to; i += 64) mine += __popcll(taken(i + lane, to));
   __syncthreads();  // (s_sum's last readers)
   if (lane == 0) s_sum[wave] = mine;
@@ -1187,7 +1188,6 @@ __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
     base += s_sum[w];
   }
   if (mine > 0) {
-#pragma unroll 4
     for (int i = from; i < to; i += 64) {
       const unsigned long long m = taken(i + lane, to);
       const int at = before + __popcll(m & ((1ull << lane) - 1));
@@ -1198,8 +1198,10 @@ __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
   for (int i = base + tid; i < a.count; i += 1024) out[i] = -1;
 }
 
+constexpr long long kMaxThreads = 0xffffffffLL;  // of a grid's dimension
+
 template <class TI, class T>
-void append_typed(AppendArgs& a, int units, hipStream_t s) {
+int append_typed(AppendArgs& a, int units, hipStream_t s) {
   constexpr int VEC = 16 / sizeof(T);  // 16-byte stores both ways
   // wide loads need whole chunks in a workgroup's heads, every chunk of the row at a multiple of its size, and rotation pairs that start at even channels of the row
   const uintptr_t align = sizeof(TI) * VEC;
@@ -1218,9 +1220,11 @@ void append_typed(AppendArgs& a, int units, hipStream_t s) {
   a.heads_per_wg = std::min((a.H + parts - 1) / parts, std::max(1, channels / a.hd));
   a.heads_per_wg = std::max(a.heads_per_wg / unit, 1) * unit;
   const dim3 grid(units, (a.H + a.heads_per_wg - 1) / a.heads_per_wg);
+  if (units * 256LL > kMaxThreads || grid.y > 65535) return 2;
   if (wide && whole) k_paged_append<TI, T, 2><<<grid, 256, 0, s>>>(a);
   else if (wide) k_paged_append<TI, T, 1><<<grid, 256, 0, s>>>(a);
   else k_paged_append<TI, T, 0><<<grid, 256, 0, s>>>(a);
+  return 0;
 }
 
 template <class T, int W, int RT>
@@ -1298,13 +1302,12 @@ int launch_paged_append(const void* k, long long k_stride, const void* v, long l
   a.keys = keys, a.values = values, a.kmin = kmin, a.kmax = kmax;
   // (context, page) pairs: each holds a token, and a context has at most two pages more than its tokens fill
   const int units = (int)std::min<long long>(n_tokens, (n_tokens >> pshift) + 2LL * B);
-  if (type == 0 && in_type == 0) append_typed<float, float>(a, units, s);
-  else if (type == 1 && in_type == 0) append_typed<float, _Float16>(a, units, s);
-  else if (type == 2 && in_type == 0) append_typed<float, __bf16>(a, units, s);
-  else if (type == 1 && in_type == 1) append_typed<_Float16, _Float16>(a, units, s);
-  else if (type == 2 && in_type == 2) append_typed<__bf16, __bf16>(a, units, s);
-  else return 1;
-  return 0;
+  if (type == 0 && in_type == 0) return append_typed<float, float>(a, units, s);
+  if (type == 1 && in_type == 0) return append_typed<float, _Float16>(a, units, s);
+  if (type == 2 && in_type == 0) return append_typed<float, __bf16>(a, units, s);
+  if (type == 1 && in_type == 1) return append_typed<_Float16, _Float16>(a, units, s);
+  if (type == 2 && in_type == 2) return append_typed<__bf16, __bf16>(a, units, s);
+  return 1;
 }
 
 long long paged_attention_workspace_floats(int B, int T, int H, int G, int hd, long long capacity, bool selected) {
@@ -1318,7 +1321,8 @@ int launch_paged_attention(const void* q, const void* keys, const void* values, 
                            hipStream_t s) {
   const int W = paged_width(hd);
   const AttPlan p = attention_plan(B, T, H, G, W, (long long)(selected ? count : slots) << pshift, selected != nullptr);
-  if (p.units * p.splits > 0x7fffffffLL || p.units / p.row_blocks * (selected ? G : T * G) > 0x7fffffffLL) return 2;
+  // (the join's rows are at most 32 times the units, 64 threads each)
+  if (p.units * p.splits * 256 > kMaxThreads || p.units * 32 * 64 > kMaxThreads) return 2;
   AttArgs a{};
   a.q = q, a.keys = keys, a.values = values, a.table = table, a.lengths = lengths, a.selected = selected;
   a.B = B, a.T = T, a.heads = H * G, a.H = H, a.G = G, a.hd = hd, a.slots = slots, a.num_pages = num_pages, a.pshift = pshift, a.count = count;
@@ -1335,7 +1339,7 @@ long long paged_select_workspace_doubles(int B, int T, int H, int slots) { retur
 
 int launch_paged_select(const void* q, const void* kmin, const void* kmax, int type, const int* table, const int* lengths, int B, int T, int H, int G,
                         int hd, int slots, int num_pages, int pshift, int count, double* work, int* out, hipStream_t s) {
-  if ((long long)B * T * H > 0x7fffffffLL || (long long)T * G > 0x7fffffffLL) return 2;
+  if ((long long)B * T * H * 1024 > kMaxThreads || (long long)T * G > 0x7fffffffLL) return 2;
   SelectArgs a{};
   a.q = q, a.kmin = kmin, a.kmax = kmax, a.table = table, a.lengths = lengths;
   a.B = B, a.T = T, a.heads = H * G, a.H = H, a.G = G, a.hd = hd, a.W = paged_width(hd), a.slots = slots, a.num_pages = num_pages, a.pshift = pshift;
@@ -1344,7 +1348,7 @@ int launch_paged_select(const void* q, const void* kmin, const void* kmax, int t
   const long long all_steps = (long long)B * H * ((slots + per_step - 1) / per_step);
   a.score_steps = (int)std::min(16LL, std::max(1LL, all_steps / 2048));  // about 8 workgroups a CU, each with its query loaded once
   a.score_blocks = (slots + per_step * a.score_steps - 1) / (per_step * a.score_steps);
-  if ((long long)B * H * a.score_blocks > 0x7fffffffLL) return 2;
+  if ((long long)B * H * a.score_blocks * 256 > kMaxThreads) return 2;
   const int blocks = B * H * a.score_blocks;
   if (type == 0) score_typed<float>(a, blocks, s);
   else if (type == 1) score_typed<_Float16>(a, blocks, s);

@@ -76,7 +76,8 @@ def call_append(**change):
 @pytest.mark.parametrize("change", [dict(page=24), dict(page=8), dict(page=512), dict(hd=0), dict(hd=257), dict(type=3), dict(type=-1), dict(in_type=1),
                                     dict(B=0), dict(slots=0), dict(slots=2 ** 28), dict(heads=0), dict(num=0), dict(tokens=-1), dict(tokens=2 ** 31),
                                     dict(axes=0), dict(axes=5), dict(rotary=21), dict(rotary=22), dict(rotary=-2), dict(base=0.0), dict(positions=None), dict(k=None), dict(keys=None),
-                                    dict(kmin=None), dict(table=None), dict(ks=-1)])
+                                    dict(kmin=None), dict(table=None), dict(ks=-1), dict(vs=2 ** 23), dict(heads=2 ** 22, hd=256, rotary=0),
+                                    dict(tokens=2 ** 31 - 1, B=2 ** 28)])
 def test_append_refuses(change):
     assert call_append(**change) != 0 and "mmf_paged_append" in _lib.last_error()
 
@@ -91,12 +92,13 @@ def call_attention(**change):
 
 @pytest.mark.parametrize("change", [dict(page=17), dict(hd=300), dict(type=7), dict(B=0), dict(T=0), dict(group=0), dict(slots=0), dict(slots=2 ** 24), dict(num=0),
                                     dict(q=None), dict(lengths=None), dict(out=None), dict(bytes=0), dict(work=None),
-                                    dict(selected=C.c_void_p(4096), count=0), dict(T=2 ** 25)])
+                                    dict(selected=C.c_void_p(4096), count=0), dict(T=2 ** 25),
+                                    dict(selected=C.c_void_p(4096), count=4, B=2 ** 15, T=2 ** 10), dict(heads=2 ** 20, B=2 ** 6, slots=4, page=16)])
 def test_attention_refuses(change):
     assert call_attention(**change) != 0 and "mmf_paged_attention" in _lib.last_error()
 
 
-@pytest.mark.parametrize("change", [dict(count=0), dict(T=0), dict(bytes=8), dict(work=None), dict(type=3), dict(page=0), dict(kmin=None), dict(group=0)])
+@pytest.mark.parametrize("change", [dict(count=0), dict(T=0), dict(bytes=8), dict(work=None), dict(type=3), dict(page=0), dict(kmin=None), dict(group=0), dict(B=2 ** 14, T=2 ** 10, bytes=1 << 50)])
 def test_selection_refuses(change):
     fake = C.c_void_p(4096)
     d = dict(q=fake, kmin=fake, kmax=fake, type=0, table=fake, lengths=fake, B=2, T=1, heads=2, group=1, hd=20, slots=100, num=4, page=16, count=3, out=fake,
