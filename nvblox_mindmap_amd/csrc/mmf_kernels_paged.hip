@@ -736,7 +736,7 @@ __global__ __launch_bounds__(256) void k_paged_join(AttArgs a, int rows_per_bloc
   f32x4 acc = {0, 0, 0, 0};
   for (int s0 = 0; s0 < ns; s0 += N) {
     const int s = min(s0 + n, ns - 1);
-    const float w = s0 + n < ns ? __shfl(f, s) : 0.0f;
+    const float fs = __shfl(f, s), w = s0 + n < ns ? fs : 0.0f;  // (every lane gives its weight, also one whose own turn is over)
     if (W != 96 || c < W / 4) acc += w * *reinterpret_cast<const f32x4*>(a.part + (first + (long long)s * rows_per_block) * W + 4 * c);
   }
 #pragma unroll
@@ -817,10 +817,11 @@ struct SelectArgs {
   int* out;        // [B, T, H, count]
 };
 
-// One summary is read once: W / 8 lanes take 8 channels of a page each, 64 / that many pages side by side in a wave, two such sets
-// at a time as 64-bit numbers in registers, all query rows over them.  The lanes' sums meet in a rotation within the 16-lane row, whose result is the same in
-// every lane.  (The 64-bit matrix instruction reaches 42 TFLOP/s here and pays for 16 rows whatever their number; four rows on
-// the vector unit cost less than the read.)
+// One summary is read once: W / 8 lanes take 8 channels of a page each, 64 / that many pages side by side in a wave, two such sets at a
+// time as 64-bit numbers in registers, all query rows over them.  The lanes' sums meet in a rotation within the 16-lane row, whose result
+// is the same in every lane.  What bounds it is half the read, half the 64-bit arithmetic (31 us for 76 MB, 4 rows of 128 channels).  Tried
+// and left: the 64-bit matrix instruction (42 TFLOP/s, and it pays for 16 rows whatever their number); 32-bit scores of all pages with a bound on
+// their error and 64-bit ones near the border alone (26 us here, but 5 to 7 more in the selection, and 7 more where rows are short).
 template <int N>
 __device__ __forceinline__ double row_rotate(double x) {  // the value N lanes on in the row of 16
   const long long u = __double_as_longlong(x);
@@ -851,8 +852,8 @@ template <class T, int W>
 __global__ __launch_bounds__(256) void k_paged_score(SelectArgs a) {
   constexpr int L = W == 96 ? 16 : W / 8, GP = 64 / L, NP = kScorePages, STEP = NP * GP, N = 16 / sizeof(T);
   __shared__ double2 s_q[kQueryRows][8][L];  // {max(q, 0), min(q, 0)} of channel 8 l + j at [row][j][l]
-  const int unit = blockIdx.x / a.score_blocks, block = blockIdx.x % a.score_blocks;
-  const int h = unit % a.H, b = unit / a.H;
+  // (heads next to each other: their summaries of a page are; 31 us against 35 for 16 contexts of up to 2048 pages)
+  const int h = blockIdx.x % a.H, block = blockIdx.x / a.H % a.score_blocks, b = blockIdx.x / a.H / a.score_blocks;
   const int P = 1 << a.pshift;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lc = lane % L, c0 = lc * 8, gp = lane / L;
   const int per_block = 4 * STEP * a.score_steps;

