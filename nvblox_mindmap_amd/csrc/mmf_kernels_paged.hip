@@ -815,6 +815,8 @@ struct SelectArgs {
   int score_blocks, score_steps;  // workgroups of a (context, head), steps of each
   double* scores;  // [B, T, H, slots]; -inf: the page is not there (entries behind the context's last page are not written)
   int* out;        // [B, T, H, count]
+  int segments;    // of a long row
+  int* chosen;     // [B, T, H, segments, count]: the best of each
 };
 
 // One summary is read once: W / 8 lanes take 8 channels of a page each, 64 / that many pages side by side in a wave, two such sets at a
@@ -957,27 +959,42 @@ __device__ __forceinline__ unsigned long long score_key(double s) {
 }
 constexpr unsigned long long kNotThere = 0x000fffffffffffffull;  // score_key(-inf)
 
-// The count best of a row, the lowest slots first among equals, written in ascending order.  The scores are rounded to 32 bits (a monotone map: they
-// sort into buckets as the scores do) and their buckets kept in LDS (the part of a row behind CAP pages is read again in each pass); the
-// scores themselves are read again only where two of a bucket have to be told apart.  A histogram over 2048 equal steps between the
+// The count best of a row, the lowest slots first among equals, written in ascending order.  The scores are rounded to 32 bits (a monotone
+// map: they sort into buckets as the scores do) and their buckets kept in LDS (the part of a row behind CAP pages is read again in each
+// pass); the scores themselves are read again only where two of a bucket have to be told apart.  A histogram over equal steps between the
 // smallest and the largest finds the bucket that holds the border; up to kFew of a bucket are ranked against each other by score and
 // slot.  A bucket with more (many near-equals, or a few scores far from the rest) is divided again by the scores' bits as integers, from
-// their highest differing bit: 11 bits a pass, so it ends.  One workgroup a row: what bounds a long row is what a CU reads and handles (29 us
-// for 31 251 pages; 6 us for 400).
-constexpr int kBuckets = 2048, kFew = 256;
-template <int CAP>
-__global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
+// their highest differing bit: 9 bits a pass and more, so it ends.
+// One workgroup a row, and what bounds a long row is what a CU reads and handles: LEVEL 1 takes segments of CAP pages, whose best LEVEL 2
+// chooses from (in the slots' order, so equals are told apart as in the row).
+constexpr int kFew = 256;
+template <int NT, int CAP, int LEVEL>
+__global__ __launch_bounds__(NT) void k_paged_select(SelectArgs a) {
+  constexpr int NW = NT / 64, NB = 2 * NT, BITS = NT == 1024 ? 11 : 9;
+  static_assert(NB == 1 << BITS && kFew <= NT, "two buckets a thread");
   __shared__ int s_bucket[CAP];
-  __shared__ int s_hist[kBuckets];
-  __shared__ unsigned long long s_lo[16], s_hi[16], s_key[kFew], s_last_key;
-  __shared__ float s_f[2][16];
-  __shared__ int s_slot[kFew], s_sum[16], s_bin, s_above, s_few, s_last_slot;
-  const long long row = blockIdx.x;
-  const int b = (int)(row / ((long long)a.T * a.H));
-  const double* __restrict__ sc = a.scores + row * a.slots;
-  int* __restrict__ out = a.out + row * a.count;
+  __shared__ int s_hist[NB];
+  __shared__ unsigned long long s_lo[NW], s_hi[NW], s_key[kFew], s_last_key;
+  __shared__ float s_f[2][NW];
+  __shared__ int s_slot[kFew], s_sum[NW], s_bin, s_above, s_few, s_last_slot;
+  const long long row = LEVEL == 1 ? blockIdx.x / a.segments : blockIdx.x;
+  const int b = (int)(row / ((long long)a.T * a.H)), first = LEVEL == 1 ? (int)(blockIdx.x % a.segments) * CAP : 0;
+  const double* __restrict__ sc = a.scores + row * a.slots + first;
+  const int* __restrict__ chosen = a.chosen + row * a.segments * a.count;
+  int* __restrict__ out = LEVEL == 1 ? a.chosen + (long long)blockIdx.x * a.count : a.out + row * a.count;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, P = 1 << a.pshift;
-  const int np = (int)min((long long)a.slots, ((long long)max(a.lengths[b], 0) + P - 1) >> a.pshift);
+  const int there = (int)min((long long)a.slots, ((long long)max(a.lengths[b], 0) + P - 1) >> a.pshift);
+  const int np = LEVEL == 1 ? min(max(there - first, 0), CAP) : LEVEL == 2 ? a.segments * a.count : there;  // entries
+  // entry i's slot and score
+  auto slot_of = [&](int i) { return LEVEL == 2 ? chosen[i] : first + i; };
+  auto score = [&](int i) {
+    if constexpr (LEVEL == 2) {
+      const int s = chosen[i];
+      return s >= 0 ? sc[s] : -(double)INFINITY;
+    } else {
+      return sc[i];
+    }
+  };
   // -inf: not there (a score below the range of 32 bits is its lowest value)
   auto rounded = [](double s) { return s == -INFINITY ? -INFINITY : s < -(double)FLT_MAX ? -FLT_MAX : (float)s; };
   const int kept = min(np, CAP);
@@ -991,20 +1008,20 @@ __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
       fhi = fmaxf(fhi, x);
     }
   };
-  for (int i0 = tid; i0 < kept; i0 += AT_ONCE * 1024) {
+  for (int i0 = tid; i0 < kept; i0 += AT_ONCE * NT) {
     double x[AT_ONCE];
 #pragma unroll
-    for (int i = 0; i < AT_ONCE; ++i) x[i] = sc[min(i0 + 1024 * i, a.slots - 1)];
+    for (int i = 0; i < AT_ONCE; ++i) x[i] = score(min(i0 + NT * i, np - 1));
 #pragma unroll
     for (int i = 0; i < AT_ONCE; ++i)
-      if (i0 + 1024 * i < kept) {
+      if (i0 + NT * i < kept) {
         const float y = rounded(x[i]);
-        s_bucket[i0 + 1024 * i] = __float_as_int(y);
+        s_bucket[i0 + NT * i] = __float_as_int(y);
         meet(y);
       }
   }
-  for (int i = tid + CAP; i < np; i += 1024) meet(rounded(sc[i]));
-  for (int i = tid; i < kBuckets; i += 1024) s_hist[i] = 0;
+  for (int i = tid + CAP; i < np; i += NT) meet(rounded(score(i)));
+  for (int i = tid; i < NB; i += NT) s_hist[i] = 0;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     flo = fminf(flo, __shfl_xor(flo, d));
@@ -1019,26 +1036,26 @@ __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
   __syncthreads();
   n = 0;
 #pragma unroll
-  for (int w = 0; w < 16; ++w) {
+  for (int w = 0; w < NW; ++w) {
     flo = fminf(flo, s_f[0][w]);
     fhi = fmaxf(fhi, s_f[1][w]);
     n += s_sum[w];
   }
   // The bucket of a score, -1: not there.  (Where the step is infinite or no number -- no two finite scores -- all of them are in bucket 0.)
-  const float inv = (float)(kBuckets - 1) / (fhi - flo);
+  const float inv = (float)(NB - 1) / (fhi - flo);
   auto bucket = [&](float x) {  // (branch-free: a row of 31 251 spends its time on these instructions)
-    int at = (int)fminf(fmaxf((x - flo) * inv, 0.0f), (float)(kBuckets - 1));
-    at = x != x ? kBuckets - 1 : at;
+    int at = (int)fminf(fmaxf((x - flo) * inv, 0.0f), (float)(NB - 1));
+    at = x != x ? NB - 1 : at;
     return x == -INFINITY ? -1 : at;
   };
 #pragma unroll 4
-  for (int i = tid; i < kept; i += 1024) {
+  for (int i = tid; i < kept; i += NT) {
     const int at = bucket(__int_as_float(s_bucket[i]));
     s_bucket[i] = at;
     if (at >= 0) atomicAdd(&s_hist[at], 1);
   }
-  for (int i = tid + CAP; i < np; i += 1024) {
-    const int at = bucket(rounded(sc[i]));
+  for (int i = tid + CAP; i < np; i += NT) {
+    const int at = bucket(rounded(score(i)));
     if (at >= 0) atomicAdd(&s_hist[at], 1);
   }
   // buckets above `border` are taken, and of those in it what is above last_key, or equal to it with a slot up to last_slot
@@ -1051,19 +1068,19 @@ __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
     // f(slot, key) over the candidates
     auto candidates = [&](auto f) {
       auto one = [&](int slot) {
-        const unsigned long long k = score_key(sc[slot]);
+        const unsigned long long k = score_key(score(slot));
         if (k >= lo && k <= hi) f(slot, k);
       };
-      for (int i = tid; i < kept; i += 1024)
+      for (int i = tid; i < kept; i += NT)
         if (s_bucket[i] == border) one(i);
-      for (int i = tid + CAP; i < np; i += 1024)
-        if (bucket(rounded(sc[i])) == border) one(i);
+      for (int i = tid + CAP; i < np; i += NT)
+        if (bucket(rounded(score(i))) == border) one(i);
     };
     for (;;) {
       if (tid == 0) s_few = 0;
       __syncthreads();
       // the bucket that holds the border: counts from the top, two buckets a thread
-      const int b1 = kBuckets - 1 - 2 * tid, h1 = s_hist[b1], h0 = s_hist[b1 - 1];
+      const int b1 = NB - 1 - 2 * tid, h1 = s_hist[b1], h0 = s_hist[b1 - 1];
       int upto = h1 + h0;
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) {
@@ -1073,7 +1090,7 @@ __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
       if (lane == 63) s_sum[wave] = upto;
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < 16; ++w) upto += w < wave ? s_sum[w] : 0;
+      for (int w = 0; w < NW; ++w) upto += w < wave ? s_sum[w] : 0;
       const int before = upto - h1 - h0;
       if (before < need && upto >= need) {
         const bool upper = before + h1 >= need;
@@ -1129,7 +1146,7 @@ __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
       }
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < 16; ++w) {
+      for (int w = 0; w < NW; ++w) {
         bl = min(bl, s_lo[w]);
         bh = max(bh, s_hi[w]);
       }
@@ -1137,16 +1154,16 @@ __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
       hi = bh;
       if (lo == hi) {  // many equals: the slot of the need-th of them
         int base = 0;
-        for (int i0 = 0; i0 < np && base < need; i0 += 1024) {
+        for (int i0 = 0; i0 < np && base < need; i0 += NT) {
           const int slot = i0 + tid;
-          const bool is = slot < np && score_key(sc[slot]) == lo;
+          const bool is = slot < np && score_key(score(slot)) == lo;
           const unsigned long long m = __ballot(is);
           __syncthreads();
           if (lane == 0) s_sum[wave] = __popcll(m);
           __syncthreads();
           int at = base;
 #pragma unroll
-          for (int w = 0; w < 16; ++w) {
+          for (int w = 0; w < NW; ++w) {
             at += w < wave ? s_sum[w] : 0;
             base += s_sum[w];
           }
@@ -1158,8 +1175,8 @@ __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
         last_slot = s_last_slot;
         break;
       }
-      shift = max(0, 64 - __clzll((long long)(hi - lo)) - 11);
-      for (int i = tid; i < kBuckets; i += 1024) s_hist[i] = 0;
+      shift = max(0, 64 - __clzll((long long)(hi - lo)) - BITS);
+      for (int i = tid; i < NB; i += NT) s_hist[i] = 0;
       __syncthreads();
       candidates([&](int, unsigned long long k) { atomicAdd(&s_hist[(int)((k - lo) >> shift)], 1); });
     }
@@ -1167,16 +1184,16 @@ __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
 
   // a wave takes a run of slots: counted, then written behind the waves before it
   auto taken = [&](int slot, int end) {
-    const int at = slot < kept ? s_bucket[min(slot, kept - 1)] : slot < end ? bucket(rounded(sc[slot])) : -1;
+    const int at = slot < kept ? s_bucket[min(slot, kept - 1)] : slot < end ? bucket(rounded(score(slot))) : -1;
     bool take = at > border && slot < end;
     if (__any(at == border && border >= 0)) {
       const bool tie = at == border && slot < end;
-      const unsigned long long k = tie ? score_key(sc[slot]) : 0;
+      const unsigned long long k = tie ? score_key(score(slot)) : 0;
       take = take || (tie && (k > last_key || (k == last_key && slot <= last_slot)));
     }
     return __ballot(take);
   };
-  const int run = ((np + 15) / 16 + 63) & ~63, from = wave * run, to = min(np, from + run);
+  const int run = ((np + NW - 1) / NW + 63) & ~63, from = wave * run, to = min(np, from + run);
   int mine = 0;
   for (int i = from; i < to; i += 64) mine += __popcll(taken(i + lane, to));
   __syncthreads();  // (s_sum's last readers)
@@ -1184,7 +1201,7 @@ __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
   __syncthreads();
   int base = 0, before = 0;
 #pragma unroll
-  for (int w = 0; w < 16; ++w) {
+  for (int w = 0; w < NW; ++w) {
     before += w < wave ? s_sum[w] : 0;
     base += s_sum[w];
   }
@@ -1192,11 +1209,11 @@ __global__ __launch_bounds__(1024) void k_paged_select(SelectArgs a) {
     for (int i = from; i < to; i += 64) {
       const unsigned long long m = taken(i + lane, to);
       const int at = before + __popcll(m & ((1ull << lane) - 1));
-      if ((m >> lane & 1) && at < a.count) out[at] = i + lane;
+      if ((m >> lane & 1) && at < a.count) out[at] = slot_of(i + lane);
       before += __popcll(m);
     }
   }
-  for (int i = base + tid; i < a.count; i += 1024) out[i] = -1;
+  for (int i = base + tid; i < a.count; i += NT) out[i] = -1;
 }
 
 constexpr long long kMaxThreads = 0xffffffffLL;  // of a grid's dimension
@@ -1336,15 +1353,20 @@ int launch_paged_attention(const void* q, const void* keys, const void* values, 
   return attention_typed<__bf16>(a, W, p.RT, blocks, s);
 }
 
-long long paged_select_workspace_doubles(int B, int T, int H, int slots) { return (long long)B * T * H * slots; }
+constexpr int kShortRow = 1536, kSegment = 4096;
+// the scores, and for rows of several segments the best of each (at most kSegment slots in all)
+long long paged_select_workspace_doubles(int B, int T, int H, int slots) {
+  return (long long)B * T * H * (slots + (slots > 2 * kSegment ? kSegment / 2 : 0));
+}
 
 int launch_paged_select(const void* q, const void* kmin, const void* kmax, int type, const int* table, const int* lengths, int B, int T, int H, int G,
                         int hd, int slots, int num_pages, int pshift, int count, double* work, int* out, hipStream_t s) {
-  if ((long long)B * T * H * 1024 > kMaxThreads || (long long)T * G > 0x7fffffffLL) return 2;
+  if ((long long)B * T * H * 1024 * (slots > 2 * kSegment ? (slots + kSegment - 1) / kSegment : 1) > kMaxThreads || (long long)T * G > 0x7fffffffLL) return 2;
   SelectArgs a{};
   a.q = q, a.kmin = kmin, a.kmax = kmax, a.table = table, a.lengths = lengths;
   a.B = B, a.T = T, a.heads = H * G, a.H = H, a.G = G, a.hd = hd, a.W = paged_width(hd), a.slots = slots, a.num_pages = num_pages, a.pshift = pshift;
   a.count = count, a.scores = work, a.out = out;
+  a.segments = (slots + kSegment - 1) / kSegment, a.chosen = (int*)(work + (long long)B * T * H * slots);
   const int L = a.W == 96 ? 16 : a.W / 8, per_step = 4 * kScorePages * (64 / L);  // pages of a workgroup's step
   const long long all_steps = (long long)B * H * ((slots + per_step - 1) / per_step);
   a.score_steps = (int)std::min(16LL, std::max(1LL, all_steps / 2048));  // about 8 workgroups a CU, each with its query loaded once
@@ -1354,9 +1376,20 @@ int launch_paged_select(const void* q, const void* kmin, const void* kmax, int t
   if (type == 0) score_typed<float>(a, blocks, s);
   else if (type == 1) score_typed<_Float16>(a, blocks, s);
   else score_typed<__bf16>(a, blocks, s);
-  // LDS for the row's scores: 16 KB leave room for two rows a CU, 128 KB hold rows of up to 32 768 pages
-  if (slots <= 4096) k_paged_select<4096><<<B * T * H, 1024, 0, s>>>(a);
-  else k_paged_select<32768><<<B * T * H, 1024, 0, s>>>(a);
+  // Short rows take four waves, where barriers are the time (336 rows of 1251 pages: 8.8 us, 12 with sixteen waves; 128 rows of up to 2048:
+  // 10.3 against 8.6).  Rows that a workgroup takes long over are cut into segments where the segments' best are few (31 251 pages, 128 of
+  // them: 18 us in two launches, 29 in one).
+  const int rows = B * T * H;
+  if (slots <= kShortRow) {
+    k_paged_select<256, kShortRow, 0><<<rows, 256, 0, s>>>(a);
+  } else if (slots <= 2 * kSegment) {
+    k_paged_select<1024, 2 * kSegment, 0><<<rows, 1024, 0, s>>>(a);
+  } else if ((long long)a.segments * count <= kSegment) {
+    k_paged_select<1024, kSegment, 1><<<rows * a.segments, 1024, 0, s>>>(a);
+    k_paged_select<1024, kSegment, 2><<<rows, 1024, 0, s>>>(a);
+  } else {
+    k_paged_select<1024, 32768, 0><<<rows, 1024, 0, s>>>(a);
+  }
   return 0;
 }
 

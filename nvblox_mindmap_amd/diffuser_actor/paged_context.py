@@ -144,6 +144,11 @@ def _attention_bytes(B, T, H, G, hd, capacity, selected) -> int:
     return int(_lib.lib().mmf_paged_attention_workspace_bytes(B, T, H, G, hd, capacity, selected))
 
 
+@functools.lru_cache(maxsize=512)
+def _select_bytes(B, T, H, slots) -> int:
+    return int(_lib.lib().mmf_paged_select_workspace_bytes(B, T, H, slots))
+
+
 def append_context(context: ContextPages, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, starts: torch.Tensor, table: torch.Tensor,
                    positions: Optional[torch.Tensor] = None, rotary_dim: Optional[int] = None, rotary_base: float = 10000.0) -> None:
     """Rows ``offsets[b] : offsets[b + 1]`` of k and v [n, kv_heads * head_dim] (the pages' type or float32; rows may be strided) become
@@ -263,7 +268,7 @@ def select_pages(q: torch.Tensor, context: ContextPages, table: torch.Tensor, le
     if not q.is_contiguous():
         q = q.contiguous()
     out = torch.empty((b, t, h, count), dtype=torch.int32, device=q.device)
-    need = 8 * b * t * h * slots
+    need = _select_bytes(b, t, h, slots)
     work = torch.empty(need, dtype=torch.uint8, device=q.device)
     _launch(index, _lib.lib().mmf_paged_select, "mmf_paged_select", q.data_ptr(), context.key_min.data_ptr(), context.key_max.data_ptr(), _TYPES[q.dtype],
             table.data_ptr(), lengths.data_ptr(), b, t, h, heads // h, hd, slots, n_pages, p, count, out.data_ptr(), work.data_ptr(), need)

@@ -317,9 +317,11 @@ def test_selection_between_scores_that_32_bits_do_not_tell_apart(dtype, pages, c
     assert got.flatten().tolist() == list(range(count))
 
 
-def test_selection_of_a_row_longer_than_its_buckets_in_lds():
-    """40 000 pages, scores in 32 bits on both sides of the border and, far out, a few that squeeze all others into one bucket."""
-    hd, pages = 16, 40000
+@pytest.mark.parametrize("pages,count", [(1536, 100), (1537, 100), (8192, 4000), (8193, 300), (9000, 2000), (40000, 300), (40000, 1000), (40000, 39999)])
+def test_selection_from_long_rows(pages, count):
+    """Rows that one workgroup takes, with its buckets in LDS or beyond them, and rows cut into segments; then a few scores far out that
+    squeeze all others into one bucket, and a query of zeros."""
+    hd = 16
     g = torch.Generator().manual_seed(4)
     low = torch.randn(pages, 1, 16, generator=g) - 1
     high = low + torch.rand(pages, 1, 16, generator=g)
@@ -328,13 +330,15 @@ def test_selection_of_a_row_longer_than_its_buckets_in_lds():
     keys = torch.zeros(pages, 1, 16, 16)
     for far in (None, 1e30):
         if far:
-            high[[7, 39999], 0, 0] = far
-            low[[7, 39999], 0, 0] = -far
+            high[[7, pages - 1], 0, 0] = far
+            low[[7, pages - 1], 0, 0] = -far
         context = P.ContextPages(keys.cuda(), keys.cuda(), low.cuda(), high.cuda(), hd)
-        got = P.select_pages(q.cuda(), context, table.cuda(), i32([16 * pages - 3]).cuda(), 1, 300)
+        got = P.select_pages(q.cuda(), context, table.cuda(), i32([16 * pages - 3]).cuda(), 1, count)
         exact = (q.double().clamp(min=0) * high[:, 0].double() + q.double().clamp(max=0) * low[:, 0].double()).sum(-1).flatten()
-        want = torch.sort(torch.sort(exact, descending=True, stable=True).indices[:300]).values.int()
+        want = torch.sort(torch.sort(exact, descending=True, stable=True).indices[:count]).values.int()
         assert torch.equal(got.cpu().flatten(), want)
+    got = P.select_pages(torch.zeros_like(q).cuda(), context, table.cuda(), i32([16 * pages]).cuda(), 1, count)
+    assert got.flatten().tolist() == list(range(count))
 
 
 # ---- together ------------------------------------------------------------------------------------------------------------------------
