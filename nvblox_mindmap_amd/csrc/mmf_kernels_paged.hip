@@ -53,7 +53,8 @@ __device__ __forceinline__ float larger(float a, float b) { return __builtin_ele
 // Token i of the rows offsets[b] .. offsets[b + 1] - 1 becomes token starts[b] + i - offsets[b] of context b.  A workgroup owns one
 // (context, page) pair and a range of heads, so a page's summary has one writer and needs no atomics; it finds its pair by a scan over
 // the contexts' page counts.  A thread takes VEC channels of VT neighbouring slots: the keys go out row by row as they came, the values
-// are transposed in its registers so that both stores are wide.
+// are transposed in its registers so that both stores are wide.  Large appends are bound by memory: 138 us for 145 000 tokens of 8 heads of 64
+// (float16, 599 MB: 4.3 TB/s), 39 us for 55 000 of 8 heads of 15 (float32, 107 MB); single tokens by the chain offsets, page, angles, store: 6 us.
 struct AppendArgs {
   const void *k, *v;
   long long k_stride, v_stride;  // below 2^23
@@ -344,7 +345,9 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
 // tiles of 32 keys in turn, each with a running maximum and sum of its own, merged through LDS at the end.  Both products run on the
 // matrix cores without a pass through LDS: S^T = K Q^T leaves lane group g of a tile with the scores of its keys, which are the operand
 // that O^T = V^T P^T takes from that lane group -- the rows of K are dealt out so that they are 8 neighbouring keys (4 in 32-bit pages), i.e. one
-// 16-byte load of a value row.  What bounds it is the single pass over keys and values.
+// 16-byte load of a value row.  What bounds it is the single pass over keys and values:
+// 237 us for 64 contexts of up to 8191 tokens, 8 heads of 128 shared by 32 (1.2 GB: 5.1 TB/s), 732 us for one of 1 000 003 (4.1 GB: 5.6 TB/s); short
+// contexts by the chain length, page, keys, values and the join: 6 + 4 us for 3080 tokens of 8 heads of 15.
 struct AttArgs {
   const void *q, *keys, *values;
   const int *table, *lengths, *selected;
