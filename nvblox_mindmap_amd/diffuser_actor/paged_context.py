@@ -149,6 +149,33 @@ def _select_bytes(B, T, H, slots) -> int:
     return int(_lib.lib().mmf_paged_select_workspace_bytes(B, T, H, slots))
 
 
+def _check_rows(context: ContextPages, k: torch.Tensor, v: torch.Tensor, positions: Optional[torch.Tensor], rotary_dim: Optional[int],
+                rotary_base: float) -> Tuple[int, int, int]:
+    """What ``append_context`` asks of the pages and the rows.  -> (axes, rotated channels, address of the positions)"""
+    keys, hd = context.keys, context.head_dim
+    _check_device(keys.get_device(), k, v, positions)
+    _check_pages(context, True)
+    h = keys.shape[1]
+    row = h * hd
+    if not (k.dim() == 2 and k.shape == v.shape and k.shape[1] == row):
+        raise ValueError(f"k and v [n, {row}]: got {tuple(k.shape)}, {tuple(v.shape)}")
+    if not (k.dtype is v.dtype and (k.dtype is keys.dtype or k.dtype is torch.float32)):
+        raise ValueError(f"k and v are {keys.dtype} or float32, both alike: got {k.dtype}, {v.dtype}")
+    n, axes, rotary, at = k.shape[0], 1, 0, 0
+    if positions is not None:
+        if not (positions.dim() == 2 and positions.shape[0] == n and 1 <= positions.shape[1] <= 4 and positions.dtype is torch.float32
+                and positions.is_contiguous()):
+            raise ValueError(f"positions [{n}, axes] float32, contiguous, 1 to 4 axes")
+        axes, rotary, at = positions.shape[1], row if rotary_dim is None else int(rotary_dim), positions.data_ptr()
+        if not (rotary > 0 and rotary % (2 * axes) == 0 and (rotary <= hd or rotary == row)):
+            raise ValueError(f"rotary_dim {rotary}: a multiple of {2 * axes}, at most head_dim {hd} or the whole row {row}")
+        if not rotary_base > 0:
+            raise ValueError("rotary_base has to be positive")
+    elif rotary_dim is not None:
+        raise ValueError("rotary_dim without positions")
+    return axes, rotary, at
+
+
 def append_context(context: ContextPages, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, starts: torch.Tensor, table: torch.Tensor,
                    positions: Optional[torch.Tensor] = None, rotary_dim: Optional[int] = None, rotary_base: float = 10000.0) -> None:
     """Rows ``offsets[b] : offsets[b + 1]`` of k and v [n, kv_heads * head_dim] (the pages' type or float32; rows may be strided) become
@@ -163,31 +190,14 @@ def append_context(context: ContextPages, k: torch.Tensor, v: torch.Tensor, offs
     read may be shared."""
     keys, hd = context.keys, context.head_dim
     index = keys.get_device()
-    _check_device(index, k, v, positions)
-    _check_pages(context, True)
+    axes, rotary, at = _check_rows(context, k, v, positions, rotary_dim, rotary_base)
     n_pages, h, p, _ = keys.shape
-    row, n = h * hd, k.shape[0]
-    if not (k.dim() == 2 and k.shape == v.shape and k.shape[1] == row):
-        raise ValueError(f"k and v [n, {row}]: got {tuple(k.shape)}, {tuple(v.shape)}")
-    if not (k.dtype is v.dtype and (k.dtype is keys.dtype or k.dtype is torch.float32)):
-        raise ValueError(f"k and v are {keys.dtype} or float32, both alike: got {k.dtype}, {v.dtype}")
+    n = k.shape[0]
     if not (_ints_ok(table, 2, index) and _ints_ok(starts, 1, index) and _ints_ok(offsets, 1, index)):
         _check_ints(keys.device, table=(table, 2), starts=(starts, 1), offsets=(offsets, 1))
     b, slots = table.shape
     if not (starts.shape[0] == b and offsets.shape[0] == b + 1):
         raise ValueError(f"{b} contexts have {b} starts and {b + 1} offsets")
-    axes, rotary, at = 1, 0, 0
-    if positions is not None:
-        if not (positions.dim() == 2 and positions.shape[0] == n and 1 <= positions.shape[1] <= 4 and positions.dtype is torch.float32
-                and positions.is_contiguous()):
-            raise ValueError(f"positions [{n}, axes] float32, contiguous, 1 to 4 axes")
-        axes, rotary, at = positions.shape[1], row if rotary_dim is None else int(rotary_dim), positions.data_ptr()
-        if not (rotary > 0 and rotary % (2 * axes) == 0 and (rotary <= hd or rotary == row)):
-            raise ValueError(f"rotary_dim {rotary}: a multiple of {2 * axes}, at most head_dim {hd} or the whole row {row}")
-        if not rotary_base > 0:
-            raise ValueError("rotary_base has to be positive")
-    elif rotary_dim is not None:
-        raise ValueError("rotary_dim without positions")
     if n == 0 or b == 0 or slots == 0:
         return
     if k.stride(1) != 1 or k.stride(0) >= 1 << 23:
@@ -382,13 +392,16 @@ class ContextMemory:
 
     def append(self, counts: Sequence[int], keys_values: Sequence[Tuple[torch.Tensor, torch.Tensor]], positions: Optional[torch.Tensor] = None,
                rotary_dim: Optional[int] = None) -> None:
-        """``counts[b]`` tokens more of every context: their (keys, values) of each layer, rows in the contexts' order, and positions."""
+        """``counts[b]`` tokens more of every context: their (keys, values) of each layer, rows in the contexts' order, and positions.
+        A call that is refused changes nothing."""
         if len(keys_values) != len(self.layers):
             raise ValueError(f"{len(self.layers)} layers' keys and values: got {len(keys_values)}")
         n = sum(int(c) for c in counts)
-        for k, v in keys_values:
+        self.pages_of.check(counts)
+        for layer, (k, v) in zip(self.layers, keys_values):  # all of it before the table counts the tokens
             if k.dim() != 2 or k.shape[0] != n or v.shape != k.shape:
                 raise ValueError(f"keys and values of {n} tokens: got {tuple(k.shape)}, {tuple(v.shape)}")
+            _check_rows(layer.pages, k, v, positions, rotary_dim, 10000.0)
         offsets, starts = self.pages_of.extend(counts)
         for layer, (k, v) in zip(self.layers, keys_values):
             append_context(layer.pages, k, v, offsets, starts, self.pages_of.table, positions, rotary_dim)

@@ -157,6 +157,16 @@ def test_memory_is_checked():
     assert m.held == (0, 0)
 
 
+def test_a_refused_append_leaves_the_memory_as_it_was():
+    m = P.ContextMemory(2, 2, 4, 2, 16, 16, device="cpu")
+    k = torch.zeros(3, 32)
+    before = m.pages_of.table.clone()
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        m.append([1, 2], [(k, k), (k, k)])
+    assert m.held == (0, 0) and m.pages_of.free_pages == 4
+    assert torch.equal(m.pages_of.table, before) and m.pages_of.lengths.tolist() == [0, 0]
+
+
 def test_model_refuses_a_memory_where_it_has_no_meaning():
     from nvblox_mindmap_amd.diffuser_actor import DiffuserActor, DiffuserActorConfig
 

@@ -156,3 +156,32 @@ def test_model_with_a_memory(fused, on):
     assert float((graphed - again)[..., :3].abs().max()) <= 5e-3 and len(model._graph_sampler._graphs) == 1
     with pytest.raises(ValueError, match="contexts"):
         run(one, model.new_context_memory(3, 64, 32))
+
+
+@pytest.mark.parametrize("case", ["width", "type", "positions", "rotary", "pool", "gradient"])
+def test_a_refused_append_leaves_the_memory_as_it_was(case):
+    memory = P.ContextMemory(2, 2, 4, 2, 16, 16)
+    first = torch.randn(5, 32, generator=torch.Generator().manual_seed(1)).cuda()
+    memory.append([3, 2], [(first, first)] * 2)
+    state = lambda: [memory.pages_of.table.clone(), memory.pages_of.lengths.clone()] + [  # noqa: E731
+        t.clone() for layer in memory.layers for t in (layer.pages.keys, layer.pages.values, layer.pages.key_min, layer.pages.key_max)]
+    before, held, free = state(), memory.held, memory.pages_of.free_pages
+    good, counts, positions, rotary = torch.ones(20, 32).cuda(), [17, 3], None, None
+    bad = good
+    if case == "width":
+        bad = torch.ones(20, 30).cuda()
+    elif case == "type":
+        bad = good.half()
+    elif case == "positions":
+        positions = torch.zeros(19, 1).cuda()
+    elif case == "rotary":
+        positions, rotary = torch.zeros(20, 3).cuda(), 16
+    elif case == "pool":
+        counts, good, bad = [60, 20], torch.ones(80, 32).cuda(), torch.ones(80, 32).cuda()
+    else:
+        bad = good.clone().requires_grad_()
+    with pytest.raises((ValueError, RuntimeError)):
+        memory.append(counts, [(good, good), (bad, bad)], positions, rotary)
+    assert memory.held == held and memory.pages_of.free_pages == free
+    for x, y in zip(state(), before):
+        assert torch.equal(x, y)
