@@ -299,8 +299,9 @@ class PageTable:
         self._free = list(range(num_pages - 1, -1, -1))
         self._pages: List[List[int]] = [[] for _ in range(contexts)]
         self._held = [0] * contexts
-        self.table = torch.full((contexts, self.slots), -1, dtype=torch.int32, device=device)
-        self.lengths = torch.zeros(contexts, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):  # (changed in place later, in whatever mode)
+            self.table = torch.full((contexts, self.slots), -1, dtype=torch.int32, device=device)
+            self.lengths = torch.zeros(contexts, dtype=torch.int32, device=device)
 
     @property
     def held(self) -> Tuple[int, ...]:
@@ -329,30 +330,39 @@ class PageTable:
     def extend(self, counts: Sequence[int]) -> Tuple[torch.Tensor, torch.Tensor]:
         """Pages for ``counts[b]`` tokens more of every context.  -> (offsets [contexts + 1], starts [contexts]) of ``append_context``;
         ``lengths`` counts the new tokens from here on.  Raises, and changes nothing, where the pool or a context's slots do not suffice."""
+        self._not_captured()
         self.check(counts)
         device = self.table.device
-        starts = torch.tensor(self._held, dtype=torch.int32).to(device)
-        offsets = [0]
-        rows, cols, ids = [], [], []
+        held, offsets = [h + int(c) for h, c in zip(self._held, counts)], [0]
+        rows, cols, ids, free = [], [], [], len(self._free)
         for b, (need, c) in enumerate(zip(self._needed(counts), counts)):
-            while len(self._pages[b]) < need:
-                page = self._free.pop()
-                rows.append(b), cols.append(len(self._pages[b])), ids.append(page)
-                self._pages[b].append(page)
-            self._held[b] += int(c)
+            for slot in range(len(self._pages[b]), need):
+                free -= 1
+                rows.append(b), cols.append(slot), ids.append(self._free[free])
             offsets.append(offsets[-1] + int(c))
+        # everything that can fail first: an error leaves the bookkeeping as it was
+        starts, lengths, ends = (torch.tensor(x, dtype=torch.int32).to(device) for x in (self._held, held, offsets))
         if ids:
             self.table[torch.tensor(rows, device=device), torch.tensor(cols, device=device)] = torch.tensor(ids, dtype=torch.int32, device=device)
-        self.lengths.copy_(torch.tensor(self._held, dtype=torch.int32))
-        return torch.tensor(offsets, dtype=torch.int32).to(device), starts
+        self.lengths.copy_(lengths)
+        for b, page in zip(rows, ids):
+            self._pages[b].append(page)
+        del self._free[free:]
+        self._held = held
+        return ends, starts
 
     def release(self, context: int) -> None:
         """Forget a context; its pages go back to the pool."""
+        self._not_captured()
+        self.table[context].fill_(-1)
+        self.lengths[context].zero_()
         self._free.extend(reversed(self._pages[context]))
         self._pages[context] = []
         self._held[context] = 0
-        self.table[context].fill_(-1)
-        self.lengths[context].zero_()
+
+    def _not_captured(self) -> None:
+        if self.table.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the page table is kept on the host: extend and release outside a captured graph (its replays read the new table)")
 
 
 class LayerContext:

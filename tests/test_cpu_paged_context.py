@@ -141,6 +141,38 @@ def test_page_table_hands_out_each_page_once():
     assert len(used) == len(set(used)) == 9
 
 
+def test_page_table_made_in_inference_mode_is_used_outside():
+    with torch.inference_mode():
+        t = P.PageTable(2, 6, 16, device="cpu")
+    t.extend([17, 1])
+    with torch.inference_mode():
+        t.extend([0, 16])
+    t.release(0)
+    assert t.held == (0, 17) and t.lengths.tolist() == [0, 17] and t.free_pages == 4
+
+
+def test_page_table_keeps_its_books_where_the_device_fails(monkeypatch):
+    t = P.PageTable(2, 6, 16, device="cpu")
+    t.extend([17, 1])
+    table, held, free, pages_ = t.table, t.held, t.free_pages, [list(p) for p in t._pages]
+
+    class Broken:
+        device, is_cuda = table.device, False
+
+        def __setitem__(self, at, value):
+            raise RuntimeError("no memory")
+
+        def __getitem__(self, at):
+            raise RuntimeError("no memory")
+
+    monkeypatch.setattr(t, "table", Broken())
+    for call in (lambda: t.extend([16, 16]), lambda: t.release(0)):
+        with pytest.raises(RuntimeError, match="no memory"):
+            call()
+    monkeypatch.setattr(t, "table", table)
+    assert t.held == held and t.free_pages == free and t._pages == pages_ and t.lengths.tolist() == [17, 1]
+
+
 def test_memory_is_checked():
     with pytest.raises(ValueError):
         P.ContextMemory(0, 1, 4, 2, 16, 16, device="cpu")

@@ -185,3 +185,19 @@ def test_a_refused_append_leaves_the_memory_as_it_was(case):
     assert memory.held == held and memory.pages_of.free_pages == free
     for x, y in zip(state(), before):
         assert torch.equal(x, y)
+
+
+def test_the_page_table_is_not_changed_in_a_capture():
+    t = P.PageTable(2, 6, 16)
+    t.extend([17, 1])
+    x = torch.zeros(64, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        x += 1
+        for call in (lambda: t.extend([1, 1]), lambda: t.release(0)):
+            with pytest.raises(RuntimeError, match="outside a captured graph"):
+                call()
+    g.replay()
+    torch.cuda.synchronize()
+    assert t.held == (17, 1) and t.lengths.tolist() == [17, 1] and t.free_pages == 3 and float(x.sum()) == 64.0
