@@ -11,6 +11,7 @@ them (float32, float16, bfloat16; no autograd; nothing synchronises, all lengths
 a graph and replayed with other lengths).  ``PageTable`` hands out a pool's pages to contexts, ``ContextMemory`` puts the table and the
 pages of a stack's layers together: what ``DiffuserActor`` keeps of earlier observations (``new_context_memory``)."""
 import functools
+import math
 from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
@@ -88,6 +89,11 @@ def _check(cond: bool, what: str) -> None:
         raise ValueError(what)
 
 
+def _check_sizes(*sizes: int) -> None:
+    if max(sizes) > 0x7fffffff:  # the library takes 32-bit sizes, and a longer one would reach it cut off
+        raise ValueError(f"sizes of a call are below 2^31: got {max(sizes)}")
+
+
 def _check_pages(c: ContextPages, summary: bool) -> None:
     if _pages_ok(c, summary):
         return
@@ -110,9 +116,9 @@ def _ints_ok(t: torch.Tensor, dim: int, index: int) -> bool:
     return t.dtype is torch.int32 and t.dim() == dim and t.get_device() == index and t.is_contiguous()
 
 
-def _check_ints(device, **ts: torch.Tensor) -> None:
+def _check_ints(keys: torch.Tensor, **ts: Tuple[torch.Tensor, int]) -> None:
     for name, (t, dim) in ts.items():
-        _check(_ints_ok(t, dim, device.index), f"{name}: a contiguous int32 tensor of {dim} dimension(s) on {device}")
+        _check(_ints_ok(t, dim, keys.get_device()), f"{name}: a contiguous int32 tensor of {dim} dimension(s) on {keys.device}")
 
 
 def _check_device(index: int, *ts: Optional[torch.Tensor]) -> None:
@@ -169,8 +175,8 @@ def _check_rows(context: ContextPages, k: torch.Tensor, v: torch.Tensor, positio
         axes, rotary, at = positions.shape[1], row if rotary_dim is None else int(rotary_dim), positions.data_ptr()
         if not (rotary > 0 and rotary % (2 * axes) == 0 and (rotary <= hd or rotary == row)):
             raise ValueError(f"rotary_dim {rotary}: a multiple of {2 * axes}, at most head_dim {hd} or the whole row {row}")
-        if not rotary_base > 0:
-            raise ValueError("rotary_base has to be positive")
+        if not 0 < rotary_base < math.inf:
+            raise ValueError("rotary_base has to be positive and finite")
     elif rotary_dim is not None:
         raise ValueError("rotary_dim without positions")
     return axes, rotary, at
@@ -193,8 +199,9 @@ def append_context(context: ContextPages, k: torch.Tensor, v: torch.Tensor, offs
     axes, rotary, at = _check_rows(context, k, v, positions, rotary_dim, rotary_base)
     n_pages, h, p, _ = keys.shape
     n = k.shape[0]
+    _check_sizes(n, *table.shape)
     if not (_ints_ok(table, 2, index) and _ints_ok(starts, 1, index) and _ints_ok(offsets, 1, index)):
-        _check_ints(keys.device, table=(table, 2), starts=(starts, 1), offsets=(offsets, 1))
+        _check_ints(keys, table=(table, 2), starts=(starts, 1), offsets=(offsets, 1))
     b, slots = table.shape
     if not (starts.shape[0] == b and offsets.shape[0] == b + 1):
         raise ValueError(f"{b} contexts have {b} starts and {b + 1} offsets")
@@ -218,8 +225,9 @@ def _check_query(q: torch.Tensor, context: ContextPages, table: torch.Tensor, le
         raise ValueError(f"q [contexts, tokens, {heads * context.head_dim}]: got {tuple(q.shape)}")
     if q.dtype is not keys.dtype:
         raise ValueError(f"q is {q.dtype}, the pages are {keys.dtype}")
+    _check_sizes(*q.shape, *table.shape)
     if not (_ints_ok(table, 2, index) and _ints_ok(lengths, 1, index)):
-        _check_ints(keys.device, table=(table, 2), lengths=(lengths, 1))
+        _check_ints(keys, table=(table, 2), lengths=(lengths, 1))
     if not table.shape[0] == q.shape[0] == lengths.shape[0]:
         raise ValueError(f"{q.shape[0]} contexts: table {tuple(table.shape)}, lengths {tuple(lengths.shape)}")
 
@@ -240,8 +248,9 @@ def context_attention(q: torch.Tensor, context: ContextPages, table: torch.Tenso
     slots, count, chosen = table.shape[1], 0, 0
     if pages is not None:
         if not _ints_ok(pages, 4, index):
-            _check_ints(keys.device, pages=(pages, 4))
+            _check_ints(keys, pages=(pages, 4))
         count, chosen = pages.shape[3], pages.data_ptr()
+        _check_sizes(count)
         if pages.shape != (b, t, h, count):
             raise ValueError(f"pages [{b}, {t}, {h}, count]: got {tuple(pages.shape)}")
     if b == 0 or t == 0 or slots == 0 or (pages is not None and count == 0):
@@ -270,6 +279,7 @@ def select_pages(q: torch.Tensor, context: ContextPages, table: torch.Tensor, le
     _check_query(q, context, table, lengths, heads, index)
     if not count > 0:
         raise ValueError("count has to be positive")
+    _check_sizes(count)
     n_pages, h, p, _ = keys.shape
     b, t, _ = q.shape
     slots = table.shape[1]

@@ -107,6 +107,91 @@ def test_selection_refuses(change):
     assert _lib.lib().mmf_paged_select(*d.values()) != 0 and "mmf_paged_select" in _lib.last_error()
 
 
+# ---- refusals of the operators' arguments, which are found on the host: on CPU tensors with the device check taken out ----
+@pytest.fixture
+def host_only(monkeypatch):
+    def reached(*args):
+        raise AssertionError("a call that has to be refused reached the library")
+
+    monkeypatch.setattr(P, "_check_device", lambda *args: None)
+    monkeypatch.setattr(P, "_launch", reached)
+
+
+def ints(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+LONG = 2 ** 31
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(k=torch.zeros(3, 41)), "k and v"),
+    (dict(k=torch.zeros(3, 40).half()), "both alike"),
+    (dict(k=torch.zeros(3, 40).half(), v=torch.zeros(3, 40).half()), "float32"),
+    (dict(v=torch.zeros(2, 40)), "k and v"),
+    (dict(starts=torch.zeros(1, dtype=torch.int64)), "starts"),
+    (dict(offsets=ints(1)), "offsets"),
+    (dict(offsets=ints(4)[::2]), "offsets"),
+    (dict(table=ints(2)), "table"),
+    (dict(table=ints(2, 2)), "starts"),
+    (dict(positions=torch.zeros(2, 1)), "positions"),
+    (dict(positions=torch.zeros(3, 5)), "positions"),
+    (dict(positions=torch.zeros(3, 1, dtype=torch.float64)), "positions"),
+    (dict(positions=torch.zeros(3, 1), rotary_dim=30), "rotary_dim"),
+    (dict(positions=torch.zeros(3, 1), rotary_dim=0), "rotary_dim"),
+    (dict(positions=torch.zeros(3, 3), rotary_dim=20), "rotary_dim"),
+    (dict(positions=torch.zeros(3, 1), rotary_base=0.0), "rotary_base"),
+    (dict(positions=torch.zeros(3, 1), rotary_base=float("inf")), "rotary_base"),
+    (dict(positions=torch.zeros(3, 1), rotary_base=float("nan")), "rotary_base"),
+    (dict(rotary_dim=20), "without positions"),
+    (dict(k=torch.zeros(1, 40).expand(LONG, 40), v=torch.zeros(1, 40).expand(LONG, 40)), "below 2"),
+    (dict(table=ints(1, 1).expand(1, LONG)), "below 2"),
+])
+def test_append_context_refuses(host_only, change, match):
+    d = dict(k=torch.zeros(3, 40), v=torch.zeros(3, 40), offsets=ints(2), starts=ints(1), table=ints(1, 2))
+    d.update(change)
+    with pytest.raises(ValueError, match=match):
+        P.append_context(pages(), **d)
+
+
+QUERY = [
+    (dict(heads=3), "multiple"),
+    (dict(heads=0), "multiple"),
+    (dict(q=torch.zeros(1, 1, 39)), "q "),
+    (dict(q=torch.zeros(1, 40)), "q "),
+    (dict(q=torch.zeros(1, 1, 40).half()), "the pages are"),
+    (dict(table=ints(2, 2)), "contexts"),
+    (dict(lengths=ints(2)), "contexts"),
+    (dict(lengths=torch.zeros(1)), "lengths"),
+    (dict(table=ints(1, 4)[:, ::2]), "table"),
+    (dict(q=torch.zeros(1, 1, 40).expand(1, LONG, 40)), "below 2"),
+    (dict(table=ints(1, 1).expand(1, LONG)), "below 2"),
+]
+
+
+def query(**change):
+    d = dict(q=torch.zeros(1, 1, 40), context=pages(), table=ints(1, 2), lengths=ints(1), heads=2)
+    d.update(change)
+    return d
+
+
+@pytest.mark.parametrize("change,match", QUERY + [
+    (dict(pages=ints(1, 1, 2)), "pages"),
+    (dict(pages=ints(1, 2, 2, 3)), "pages"),
+    (dict(pages=torch.zeros(1, 1, 2, 3, dtype=torch.int64)), "pages"),
+])
+def test_context_attention_refuses(host_only, change, match):
+    with pytest.raises(ValueError, match=match):
+        P.context_attention(**query(**change))
+
+
+@pytest.mark.parametrize("change,match", QUERY + [(dict(count=0), "count"), (dict(count=-1), "count"), (dict(count=LONG), "below 2"),
+                                                  (dict(count=2 ** 32 + 5), "below 2"), (dict(context=pages(key_min=None)), "key_min")])
+def test_select_pages_refuses(host_only, change, match):
+    with pytest.raises(ValueError, match=match):
+        P.select_pages(**{**query(count=2), **query(**change)} if "count" in change else {**query(**change), "count": 2})
+
+
 def test_workspace_sizes():
     L = _lib.lib()
     assert L.mmf_paged_select_workspace_bytes(2, 3, 4, 5) >= 8 * 120
