@@ -89,9 +89,11 @@ def _check(cond: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _check_sizes(*sizes: int) -> None:
-    if max(sizes) > 0x7fffffff:  # the library takes 32-bit sizes, and a longer one would reach it cut off
-        raise ValueError(f"sizes of a call are below 2^31: got {max(sizes)}")
+_LONG = 31  # sizes of a call, or-ed together and shifted: the library takes 32-bit sizes, and a longer one would reach it cut off
+
+
+def _too_long(*sizes: int) -> ValueError:
+    return ValueError(f"sizes of a call are below 2^31: got {max(sizes)}")
 
 
 def _check_pages(c: ContextPages, summary: bool) -> None:
@@ -199,10 +201,11 @@ def append_context(context: ContextPages, k: torch.Tensor, v: torch.Tensor, offs
     axes, rotary, at = _check_rows(context, k, v, positions, rotary_dim, rotary_base)
     n_pages, h, p, _ = keys.shape
     n = k.shape[0]
-    _check_sizes(n, *table.shape)
     if not (_ints_ok(table, 2, index) and _ints_ok(starts, 1, index) and _ints_ok(offsets, 1, index)):
         _check_ints(keys, table=(table, 2), starts=(starts, 1), offsets=(offsets, 1))
     b, slots = table.shape
+    if (n | b | slots) >> _LONG:
+        raise _too_long(n, b, slots)
     if not (starts.shape[0] == b and offsets.shape[0] == b + 1):
         raise ValueError(f"{b} contexts have {b} starts and {b + 1} offsets")
     if n == 0 or b == 0 or slots == 0:
@@ -225,9 +228,11 @@ def _check_query(q: torch.Tensor, context: ContextPages, table: torch.Tensor, le
         raise ValueError(f"q [contexts, tokens, {heads * context.head_dim}]: got {tuple(q.shape)}")
     if q.dtype is not keys.dtype:
         raise ValueError(f"q is {q.dtype}, the pages are {keys.dtype}")
-    _check_sizes(*q.shape, *table.shape)
     if not (_ints_ok(table, 2, index) and _ints_ok(lengths, 1, index)):
         _check_ints(keys, table=(table, 2), lengths=(lengths, 1))
+    b, t, row = q.shape
+    if (b | t | row | table.shape[1]) >> _LONG:
+        raise _too_long(b, t, row, table.shape[1])
     if not table.shape[0] == q.shape[0] == lengths.shape[0]:
         raise ValueError(f"{q.shape[0]} contexts: table {tuple(table.shape)}, lengths {tuple(lengths.shape)}")
 
@@ -250,7 +255,8 @@ def context_attention(q: torch.Tensor, context: ContextPages, table: torch.Tenso
         if not _ints_ok(pages, 4, index):
             _check_ints(keys, pages=(pages, 4))
         count, chosen = pages.shape[3], pages.data_ptr()
-        _check_sizes(count)
+        if count >> _LONG:
+            raise _too_long(count)
         if pages.shape != (b, t, h, count):
             raise ValueError(f"pages [{b}, {t}, {h}, count]: got {tuple(pages.shape)}")
     if b == 0 or t == 0 or slots == 0 or (pages is not None and count == 0):
@@ -279,7 +285,8 @@ def select_pages(q: torch.Tensor, context: ContextPages, table: torch.Tensor, le
     _check_query(q, context, table, lengths, heads, index)
     if not count > 0:
         raise ValueError("count has to be positive")
-    _check_sizes(count)
+    if count >> _LONG:
+        raise _too_long(count)
     n_pages, h, p, _ = keys.shape
     b, t, _ = q.shape
     slots = table.shape[1]

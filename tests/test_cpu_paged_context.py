@@ -145,7 +145,7 @@ LONG = 2 ** 31
     (dict(positions=torch.zeros(3, 1), rotary_base=float("nan")), "rotary_base"),
     (dict(rotary_dim=20), "without positions"),
     (dict(k=torch.zeros(1, 40).expand(LONG, 40), v=torch.zeros(1, 40).expand(LONG, 40)), "below 2"),
-    (dict(table=ints(1, 1).expand(1, LONG)), "below 2"),
+    (dict(table=torch.empty(1, LONG, dtype=torch.int32)), "below 2"),
 ])
 def test_append_context_refuses(host_only, change, match):
     d = dict(k=torch.zeros(3, 40), v=torch.zeros(3, 40), offsets=ints(2), starts=ints(1), table=ints(1, 2))
@@ -165,7 +165,7 @@ QUERY = [
     (dict(lengths=torch.zeros(1)), "lengths"),
     (dict(table=ints(1, 4)[:, ::2]), "table"),
     (dict(q=torch.zeros(1, 1, 40).expand(1, LONG, 40)), "below 2"),
-    (dict(table=ints(1, 1).expand(1, LONG)), "below 2"),
+    (dict(table=torch.empty(1, LONG, dtype=torch.int32)), "below 2"),
 ]
 
 
