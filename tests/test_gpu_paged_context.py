@@ -317,7 +317,7 @@ def test_selection_between_scores_that_32_bits_do_not_tell_apart(dtype, pages, c
     assert got.flatten().tolist() == list(range(count))
 
 
-@pytest.mark.parametrize("pages,count", [(1536, 100), (1537, 100), (8192, 4000), (8193, 300), (9000, 2000), (40000, 300), (40000, 1000), (40000, 39999)])
+@pytest.mark.parametrize("pages,count", [(1536, 100), (1537, 100), (8192, 4000), (8193, 300), (9000, 2000), (40000, 100), (31251, 128), (40000, 300), (40000, 1000), (40000, 39999)])
 def test_selection_from_long_rows(pages, count):
     """Rows that one workgroup takes, with its buckets in LDS or beyond them, and rows cut into segments; then a few scores far out that
     squeeze all others into one bucket, and a query of zeros."""
