@@ -65,17 +65,18 @@ def allocate_pages(num_pages: int, kv_heads: int, head_dim: int, page_size: int 
 
 # ---- checks: one expression on the way to the kernel (a call's host time is a good part of a small call), the reason only where it fails ----
 def _pages_ok(c: ContextPages, summary: bool) -> bool:
-    k, v = c.keys, c.values
-    if k.dim() != 4:
+    k, v, lo, hi, hd = c
+    shape = k.shape
+    if len(shape) != 4:
         return False
-    n, h, p, w = k.shape
+    n, h, p, w = shape
     dtype, index = k.dtype, k.get_device()
-    ok = (dtype in _TYPES and v.dtype is dtype and p in PAGE_SIZES and n > 0 and h > 0 and 1 <= c.head_dim <= 256 and w == _WIDTH_OF[c.head_dim]
+    ok = (dtype in _TYPES and v.dtype is dtype and p in PAGE_SIZES and n > 0 and h > 0 and 1 <= hd <= 256 and w == _WIDTH_OF[hd]
           and v.shape == (n, h, w, p) and k.is_contiguous() and v.is_contiguous() and v.get_device() == index
           and not (k.data_ptr() | v.data_ptr()) & 15)
     if ok and summary:
-        lo, hi = c.key_min, c.key_max
-        ok = (lo is not None and hi is not None and lo.shape == (n, h, w) and hi.shape == (n, h, w) and lo.dtype is dtype and hi.dtype is dtype
+        shape = (n, h, w)
+        ok = (lo is not None and hi is not None and lo.shape == shape and hi.shape == shape and lo.dtype is dtype and hi.dtype is dtype
               and lo.is_contiguous() and hi.is_contiguous() and lo.get_device() == index and hi.get_device() == index
               and not (lo.data_ptr() | hi.data_ptr()) & 15)
     return ok
@@ -158,30 +159,32 @@ def _select_bytes(B, T, H, slots) -> int:
 
 
 def _check_rows(context: ContextPages, k: torch.Tensor, v: torch.Tensor, positions: Optional[torch.Tensor], rotary_dim: Optional[int],
-                rotary_base: float) -> Tuple[int, int, int]:
-    """What ``append_context`` asks of the pages and the rows.  -> (axes, rotated channels, address of the positions)"""
+                rotary_base: float) -> Tuple[int, int, int, int]:
+    """What ``append_context`` asks of the pages and the rows.  -> (rows, axes, rotated channels, address of the positions)"""
     keys, hd = context.keys, context.head_dim
     _check_device(keys.get_device(), k, v, positions)
-    _check_pages(context, True)
-    h = keys.shape[1]
-    row = h * hd
-    if not (k.dim() == 2 and k.shape == v.shape and k.shape[1] == row):
+    if not _pages_ok(context, True):
+        _check_pages(context, True)
+    row = keys.shape[1] * hd
+    shape = k.shape
+    if not (len(shape) == 2 and shape[1] == row and v.shape == shape):
         raise ValueError(f"k and v [n, {row}]: got {tuple(k.shape)}, {tuple(v.shape)}")
-    if not (k.dtype is v.dtype and (k.dtype is keys.dtype or k.dtype is torch.float32)):
+    dtype, n = k.dtype, shape[0]
+    if not (v.dtype is dtype and (dtype is keys.dtype or dtype is torch.float32)):
         raise ValueError(f"k and v are {keys.dtype} or float32, both alike: got {k.dtype}, {v.dtype}")
-    n, axes, rotary, at = k.shape[0], 1, 0, 0
-    if positions is not None:
-        if not (positions.dim() == 2 and positions.shape[0] == n and 1 <= positions.shape[1] <= 4 and positions.dtype is torch.float32
-                and positions.is_contiguous()):
-            raise ValueError(f"positions [{n}, axes] float32, contiguous, 1 to 4 axes")
-        axes, rotary, at = positions.shape[1], row if rotary_dim is None else int(rotary_dim), positions.data_ptr()
-        if not (rotary > 0 and rotary % (2 * axes) == 0 and (rotary <= hd or rotary == row)):
-            raise ValueError(f"rotary_dim {rotary}: a multiple of {2 * axes}, at most head_dim {hd} or the whole row {row}")
-        if not 0 < rotary_base < math.inf:
-            raise ValueError("rotary_base has to be positive and finite")
-    elif rotary_dim is not None:
-        raise ValueError("rotary_dim without positions")
-    return axes, rotary, at
+    if positions is None:
+        if rotary_dim is not None:
+            raise ValueError("rotary_dim without positions")
+        return n, 1, 0, 0
+    shape = positions.shape
+    if not (len(shape) == 2 and shape[0] == n and 1 <= shape[1] <= 4 and positions.dtype is torch.float32 and positions.is_contiguous()):
+        raise ValueError(f"positions [{n}, axes] float32, contiguous, 1 to 4 axes")
+    axes, rotary = shape[1], row if rotary_dim is None else int(rotary_dim)
+    if not (rotary > 0 and rotary % (2 * axes) == 0 and (rotary <= hd or rotary == row)):
+        raise ValueError(f"rotary_dim {rotary}: a multiple of {2 * axes}, at most head_dim {hd} or the whole row {row}")
+    if not 0 < rotary_base < math.inf:
+        raise ValueError("rotary_base has to be positive and finite")
+    return n, axes, rotary, positions.data_ptr()
 
 
 def append_context(context: ContextPages, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, starts: torch.Tensor, table: torch.Tensor,
@@ -196,45 +199,53 @@ def append_context(context: ContextPages, k: torch.Tensor, v: torch.Tensor, offs
 
     A page gets tokens of one context in a call (two that append to one page in the same call leave it undefined); pages that are only
     read may be shared."""
-    keys, hd = context.keys, context.head_dim
+    keys, values, low, high, hd = context
+    n, axes, rotary, at = _check_rows(context, k, v, positions, rotary_dim, rotary_base)
     index = keys.get_device()
-    axes, rotary, at = _check_rows(context, k, v, positions, rotary_dim, rotary_base)
-    n_pages, h, p, _ = keys.shape
-    n = k.shape[0]
     if not (_ints_ok(table, 2, index) and _ints_ok(starts, 1, index) and _ints_ok(offsets, 1, index)):
         _check_ints(keys, table=(table, 2), starts=(starts, 1), offsets=(offsets, 1))
+    n_pages, h, p, _ = keys.shape
     b, slots = table.shape
     if (n | b | slots) >> _LONG:
         raise _too_long(n, b, slots)
-    if not (starts.shape[0] == b and offsets.shape[0] == b + 1):
+    if not (starts.numel() == b and offsets.numel() == b + 1):
         raise ValueError(f"{b} contexts have {b} starts and {b + 1} offsets")
     if n == 0 or b == 0 or slots == 0:
         return
-    if k.stride(1) != 1 or k.stride(0) >= 1 << 23:
-        k = k.contiguous()
-    if v.stride(1) != 1 or v.stride(0) >= 1 << 23:
-        v = v.contiguous()
-    _launch(index, _lib.lib().mmf_paged_append, "mmf_paged_append", k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), _TYPES[k.dtype], n, at, axes,
+    (k_stride, k_step), (v_stride, v_step) = k.stride(), v.stride()
+    if k_step != 1 or k_stride >= 1 << 23:
+        k, k_stride = k.contiguous(), h * hd
+    if v_step != 1 or v_stride >= 1 << 23:
+        v, v_stride = v.contiguous(), h * hd
+    _launch(index, _lib.lib().mmf_paged_append, "mmf_paged_append", k.data_ptr(), k_stride, v.data_ptr(), v_stride, _TYPES[k.dtype], n, at, axes,
             rotary, rotary_base, offsets.data_ptr(), starts.data_ptr(), table.data_ptr(), b, slots, p, h, hd, n_pages, _TYPES[keys.dtype], keys.data_ptr(),
-            context.values.data_ptr(), context.key_min.data_ptr(), context.key_max.data_ptr())
+            values.data_ptr(), low.data_ptr(), high.data_ptr())
 
 
-def _check_query(q: torch.Tensor, context: ContextPages, table: torch.Tensor, lengths: torch.Tensor, heads: int, index: int) -> None:
+def _check_query(q: torch.Tensor, context: ContextPages, table: torch.Tensor, lengths: torch.Tensor, heads: int, summary: bool) -> Tuple[int, int, int]:
+    """What the attention and the selection ask of pages, query and table.  -> (contexts, tokens, slots)"""
     keys = context.keys
+    index = keys.get_device()
+    _check_device(index, q)
+    if not _pages_ok(context, summary):
+        _check_pages(context, summary)
     h = keys.shape[1]
     if not (heads > 0 and heads % h == 0):
         raise ValueError(f"heads {heads}: a multiple of the {h} key-value heads")
-    if not (q.dim() == 3 and q.shape[2] == heads * context.head_dim):
-        raise ValueError(f"q [contexts, tokens, {heads * context.head_dim}]: got {tuple(q.shape)}")
+    shape, row = q.shape, heads * context.head_dim
+    if not (len(shape) == 3 and shape[2] == row):
+        raise ValueError(f"q [contexts, tokens, {row}]: got {tuple(shape)}")
     if q.dtype is not keys.dtype:
         raise ValueError(f"q is {q.dtype}, the pages are {keys.dtype}")
     if not (_ints_ok(table, 2, index) and _ints_ok(lengths, 1, index)):
         _check_ints(keys, table=(table, 2), lengths=(lengths, 1))
-    b, t, row = q.shape
-    if (b | t | row | table.shape[1]) >> _LONG:
-        raise _too_long(b, t, row, table.shape[1])
-    if not table.shape[0] == q.shape[0] == lengths.shape[0]:
-        raise ValueError(f"{q.shape[0]} contexts: table {tuple(table.shape)}, lengths {tuple(lengths.shape)}")
+    b, t, _ = shape
+    contexts, slots = table.shape
+    if (b | t | row | slots) >> _LONG:
+        raise _too_long(b, t, row, slots)
+    if not contexts == b == lengths.numel():
+        raise ValueError(f"{b} contexts: table {tuple(table.shape)}, lengths {tuple(lengths.shape)}")
+    return b, t, slots
 
 
 def context_attention(q: torch.Tensor, context: ContextPages, table: torch.Tensor, lengths: torch.Tensor, heads: int,
@@ -243,14 +254,11 @@ def context_attention(q: torch.Tensor, context: ContextPages, table: torch.Tenso
     [contexts, T, heads * head_dim] of the pages' type, rotated by the caller (``fused_ops.rotary_apply``, ``q_block``); query head i reads
     key-value head i // (heads / kv_heads).  ``pages`` [contexts, T, kv_heads, count] int32 (``select_pages``): over the tokens of these
     table slots only; an entry outside the table holds nothing, none may stand twice.  Zeros where there is no token.  -> [contexts, T, heads * head_dim]."""
-    keys, hd = context.keys, context.head_dim
+    b, t, slots = _check_query(q, context, table, lengths, heads, False)
+    keys, values, _, _, hd = context
     index = keys.get_device()
-    _check_device(index, q)
-    _check_pages(context, False)
-    _check_query(q, context, table, lengths, heads, index)
     n_pages, h, p, _ = keys.shape
-    b, t, _ = q.shape
-    slots, count, chosen = table.shape[1], 0, 0
+    count, chosen = 0, 0
     if pages is not None:
         if not _ints_ok(pages, 4, index):
             _check_ints(keys, pages=(pages, 4))
@@ -267,7 +275,7 @@ def context_attention(q: torch.Tensor, context: ContextPages, table: torch.Tenso
     need = _attention_bytes(b, t, h, heads // h, hd, (slots if pages is None else count) * p, int(pages is not None))
     # per call, from torch's caching allocator: safe inside a captured graph (its private pool) and across streams
     work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _launch(index, _lib.lib().mmf_paged_attention, "mmf_paged_attention", q.data_ptr(), keys.data_ptr(), context.values.data_ptr(), _TYPES[q.dtype],
+    _launch(index, _lib.lib().mmf_paged_attention, "mmf_paged_attention", q.data_ptr(), keys.data_ptr(), values.data_ptr(), _TYPES[q.dtype],
             table.data_ptr(), lengths.data_ptr(), chosen, count, b, t, h, heads // h, hd, slots, n_pages, p, hd ** -0.5 if scale is None else scale,
             out.data_ptr(), work.data_ptr() if need else 0, need)
     return out
@@ -278,18 +286,14 @@ def select_pages(q: torch.Tensor, context: ContextPages, table: torch.Tensor, le
     [contexts, T, kv_heads, count] int32, ascending, filled up with -1 -- the ``pages`` of ``context_attention``.  A page's score is
     sum_c max(q_c, 0) key_max_c + min(q_c, 0) key_min_c, which no key of the page exceeds, the largest over the query heads that share the
     key-value head; taken in 64 bits, the lower slot first among equals."""
-    keys, hd = context.keys, context.head_dim
+    b, t, slots = _check_query(q, context, table, lengths, heads, True)
+    keys, _, low, high, hd = context
     index = keys.get_device()
-    _check_device(index, q)
-    _check_pages(context, True)
-    _check_query(q, context, table, lengths, heads, index)
     if not count > 0:
         raise ValueError("count has to be positive")
     if count >> _LONG:
         raise _too_long(count)
     n_pages, h, p, _ = keys.shape
-    b, t, _ = q.shape
-    slots = table.shape[1]
     if b == 0 or t == 0 or slots == 0:
         return torch.full((b, t, h, count), -1, dtype=torch.int32, device=q.device)
     if not q.is_contiguous():
@@ -297,7 +301,7 @@ def select_pages(q: torch.Tensor, context: ContextPages, table: torch.Tensor, le
     out = torch.empty((b, t, h, count), dtype=torch.int32, device=q.device)
     need = _select_bytes(b, t, h, slots)
     work = torch.empty(need, dtype=torch.uint8, device=q.device)
-    _launch(index, _lib.lib().mmf_paged_select, "mmf_paged_select", q.data_ptr(), context.key_min.data_ptr(), context.key_max.data_ptr(), _TYPES[q.dtype],
+    _launch(index, _lib.lib().mmf_paged_select, "mmf_paged_select", q.data_ptr(), low.data_ptr(), high.data_ptr(), _TYPES[q.dtype],
             table.data_ptr(), lengths.data_ptr(), b, t, h, heads // h, hd, slots, n_pages, p, count, out.data_ptr(), work.data_ptr(), need)
     return out
 
