@@ -1061,6 +1061,7 @@ __global__ __launch_bounds__(NT) void k_paged_select(SelectArgs a) {
     const int at = bucket(rounded(score(i)));
     if (at >= 0) atomicAdd(&s_hist[at], 1);
   }
+  __syncthreads();  // (from here on a wave reads buckets that others wrote, also where the border below is not looked for)
   // buckets above `border` are taken, and of those in it what is above last_key, or equal to it with a slot up to last_slot
   int border = -1, last_slot = 0x7fffffff;
   unsigned long long last_key = 0;
