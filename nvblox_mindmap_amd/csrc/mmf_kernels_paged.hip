@@ -1108,7 +1108,8 @@ __global__ __launch_bounds__(NT) void k_paged_select(SelectArgs a) {
         border = bin;
       } else {
         const unsigned long long from = lo + ((unsigned long long)bin << shift);
-        hi = min(hi, from + ((1ull << shift) - 1));
+        const unsigned long long rest = (1ull << shift) - 1;  // (from + rest may pass 2^64: hi is the key of a NaN)
+        hi = hi - from > rest ? from + rest : hi;
         lo = from;
       }
       if (inside <= kFew) {

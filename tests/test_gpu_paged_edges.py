@@ -2,6 +2,8 @@
 lengths far outside the table, launch forms of large calls (against the 64-bit restatement of paged_reference)."""
 import math
 
+import math
+
 import pytest
 import torch
 
@@ -41,3 +43,23 @@ def test_a_row_that_is_taken_whole(slots, held, count):
         there = (table[b, :held] >= 0).nonzero().flatten().to(torch.int32)
         want = torch.cat([there, torch.full((count - len(there),), -1, dtype=torch.int32)])
         assert torch.equal(got[b], want.expand(T, H, count)), b
+
+
+# pages, how many of them have no number for a score, how many share the largest score, count
+@pytest.mark.parametrize("pages,nans,tops,count", [(1000, 300, 1, 7), (1000, 300, 1, 300), (1000, 300, 1, 299), (1000, 300, 1, 500), (700, 5, 300, 2), (700, 5, 300, 5), (700, 5, 300, 6), (700, 5, 300, 400),
+                                                   (5000, 600, 2, 333), (5000, 3, 900, 3), (40000, 2000, 1, 100), (40000, 5000, 300, 4500), (40000, 9, 5000, 8), (40000, 9, 9000, 5000)])
+def test_pages_whose_score_is_not_a_number_come_first(pages, nans, tops, count):
+    """Several hundred of them, or of the largest number, share the bucket that holds the border: it is divided again, up to the very end of the keys' range."""
+    hd, g = 16, torch.Generator().manual_seed(pages + nans)
+    high = torch.rand(pages, 1, 16, generator=g)
+    q = torch.rand(1, 1, hd, generator=g) + 0.1
+    place = torch.randperm(pages - 1, generator=g) + 1
+    best = torch.cat([torch.zeros(1, dtype=torch.long), place[:tops - 1]])  # slot 0 among them
+    high[best] = 1.5
+    none = place[tops:tops + nans]
+    high[none, 0, 3] = math.nan
+    table = torch.arange(pages, dtype=torch.int32)[None].contiguous()
+    got = P.select_pages(q.cuda(), summaries(high, high, hd), table.cuda(), i32([16 * pages]).cuda(), 1, count).cpu().flatten()
+    score = (q.double() * high[:, 0].double()).sum(-1).flatten()
+    order = torch.sort(torch.where(torch.isnan(score), math.inf, score), descending=True, stable=True).indices
+    assert torch.equal(got, torch.sort(order[:count]).values.int())
