@@ -485,7 +485,7 @@ __global__ __launch_bounds__(256) void k_paged_attention(AttArgs a) {
       const int logical = u.sel ? u.sel[e0 + i] : e0 + i;
       int page = -1, valid = 0;
       if (logical >= 0 && logical < a.slots) page = a.table[(long long)u.b * a.slots + logical];
-      if (page >= 0 && page < a.num_pages) valid = min(max(a.lengths[u.b] - (logical << a.pshift), 0), P);
+      if (page >= 0 && page < a.num_pages) valid = min(max(max(a.lengths[u.b], 0) - (logical << a.pshift), 0), P);
       else page = 0;
       s_page[i] = page;
       s_valid[i] = valid;

@@ -63,3 +63,20 @@ def test_pages_whose_score_is_not_a_number_come_first(pages, nans, tops, count):
     score = (q.double() * high[:, 0].double()).sum(-1).flatten()
     order = torch.sort(torch.where(torch.isnan(score), math.inf, score), descending=True, stable=True).indices
     assert torch.equal(got, torch.sort(order[:count]).values.int())
+
+
+@pytest.mark.parametrize("n", [-2 ** 31, -2 ** 31 + 1, -2 ** 31 + 47, -5, 2 ** 31 - 1])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_lengths_far_outside_the_table(n, dtype):
+    """A length is clamped to what the table holds, on every path; below zero there is no token."""
+    pages = R.make_pages(6, 2, 16, 16, dtype)
+    table, q = i32([[2, 4, 0, 1, 5]]), torch.randn(1, 2, 32, generator=torch.Generator().manual_seed(1)).to(dtype)
+    context = P.ContextPages(*(t.cuda() for t in pages), 16)
+    lengths, held = i32([n]).cuda(), 0 if n < 0 else 80
+    selected = i32([0, 1, 3, 4]).expand(1, 2, 2, 4).contiguous()
+    for chosen in (None, selected):
+        got = P.context_attention(q.cuda(), context, table.cuda(), lengths, 2, pages=None if chosen is None else chosen.cuda()).cpu()
+        want, bound = R.attention(q, pages, table, [held], 2, 16, selected=chosen)
+        assert bool(((got.double() - want).abs() <= bound).all())
+    got = P.select_pages(q.cuda(), context, table.cuda(), lengths, 2, 3).cpu()
+    assert torch.equal(got, R.select(q, pages[2], pages[3], table, [held], 16, 2, 16, 3))
