@@ -617,7 +617,7 @@ int mmf_paged_attention(const void* q_dev, const void* keys_dev, const void* val
 /* The `count` table slots of every query token and key-value head with the highest scores, ascending, filled up with -1: selected
  * [B, T, kv_heads, count].  A page's score is sum_c max(q_c, 0) key_max_c + min(q_c, 0) key_min_c -- no key of the page has a larger
  * product with q --, the largest over the `group` query heads; in 64 bits, the lower slot first among equals.  A page whose score is not
- * a number comes first.  workspace: mmf_paged_select_workspace_bytes bytes. */
+ * a number comes first.  0 < count < 2^30.  workspace: mmf_paged_select_workspace_bytes bytes. */
 int64_t mmf_paged_select_workspace_bytes(int B, int T, int kv_heads, int slots);
 int mmf_paged_select(const void* q_dev, const void* key_min_dev, const void* key_max_dev, int type, const int32_t* table_dev,
                      const int32_t* lengths_dev, int B, int T, int kv_heads, int group, int head_dim, int slots, int num_pages, int page_size,

@@ -647,6 +647,7 @@ int mmf_paged_select(const void* q, const void* key_min, const void* key_max, in
   if (const char* e = paged_shape_error(type, B, slots, page_size, kv_heads, head_dim, num_pages)) return paged_fail(name, e);
   if (!q || !key_min || !key_max || !table || !lengths || !selected || !workspace) return paged_fail(name, "null pointer");
   if (T <= 0 || group <= 0 || count <= 0 || (int64_t)kv_heads * group * head_dim > 0x7fffffffLL) return paged_fail(name, "positive T, group and count");
+  if (count >= (1 << 30)) return paged_fail(name, "count is below 2^30");
   if (workspace_bytes < mmf_paged_select_workspace_bytes(B, T, kv_heads, slots)) return paged_fail(name, "workspace smaller than mmf_paged_select_workspace_bytes");
   if (launch_paged_select(q, key_min, key_max, type, table, lengths, B, T, kv_heads, group, head_dim, slots, num_pages, page_shift(page_size), count,
                           (double*)workspace, selected, (hipStream_t)stream) != 0)

@@ -291,8 +291,8 @@ def select_pages(q: torch.Tensor, context: ContextPages, table: torch.Tensor, le
     index = keys.get_device()
     if not count > 0:
         raise ValueError("count has to be positive")
-    if count >> _LONG:
-        raise _too_long(count)
+    if count >> 30:
+        raise ValueError(f"count is below 2^30: got {count}")
     n_pages, h, p, _ = keys.shape
     if b == 0 or t == 0 or slots == 0:
         return torch.full((b, t, h, count), -1, dtype=torch.int32, device=q.device)

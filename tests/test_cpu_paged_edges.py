@@ -1,0 +1,37 @@
+"""What the paged context operators and their bookkeeping do at the edges, where no GPU is needed."""
+import ctypes as C
+
+import pytest
+import torch
+
+from nvblox_mindmap_amd import _lib
+from nvblox_mindmap_amd.diffuser_actor import paged_context as P
+
+
+def pages():
+    low, high = torch.zeros(4, 2, 32), torch.zeros(4, 2, 32)
+    return P.ContextPages(torch.zeros(4, 2, 16, 32), torch.zeros(4, 2, 32, 16), low, high, 20)
+
+
+def ints(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+@pytest.fixture
+def host_only(monkeypatch):
+    """The operators' checks on CPU tensors: the calls that pass them are collected instead of launched."""
+    calls = []
+    monkeypatch.setattr(P, "_check_device", lambda *args: None)
+    monkeypatch.setattr(P, "_launch", lambda *args: calls.append(args))
+    return calls
+
+
+@pytest.mark.parametrize("count", [2 ** 30, 2 ** 31 - 1])
+def test_selection_refuses_counts_that_its_index_would_pass(host_only, count):
+    """The fill behind a row's last page steps on from an index below count: it has to stay in 32 bits."""
+    fake = C.c_void_p(4096)
+    rc = _lib.lib().mmf_paged_select(fake, fake, fake, 0, fake, fake, 1, 1, 1, 1, 20, 100, 4, 16, count, fake, fake, 1 << 30, None)
+    assert rc != 0 and "count is below 2^30" in _lib.last_error()
+    with pytest.raises(ValueError, match="below 2"):
+        P.select_pages(torch.zeros(1, 1, 40), pages(), ints(1, 2), ints(1), 2, count)
+    assert not host_only
