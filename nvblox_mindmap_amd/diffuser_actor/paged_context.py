@@ -372,6 +372,16 @@ class PageTable:
         self._held = held
         return ends, starts
 
+    def _take_back(self, held: Sequence[int]) -> None:
+        """Every context holds ``held[b]`` tokens again: undoes an ``extend`` whose tokens could not be stored."""
+        self.lengths.copy_(torch.tensor(held, dtype=torch.int32))
+        for b in reversed(range(len(held))):  # (the pool's order as it was)
+            keep = -(-held[b] // self.page_size)
+            self.table[b, keep:].fill_(-1)
+            self._free.extend(reversed(self._pages[b][keep:]))
+            del self._pages[b][keep:]
+        self._held = list(held)
+
     def release(self, context: int) -> None:
         """Forget a context; its pages go back to the pool."""
         self._not_captured()
@@ -433,9 +443,14 @@ class ContextMemory:
             if k.dim() != 2 or k.shape[0] != n or v.shape != k.shape:
                 raise ValueError(f"keys and values of {n} tokens: got {tuple(k.shape)}, {tuple(v.shape)}")
             _check_rows(layer.pages, k, v, positions, rotary_dim, 10000.0)
+        held = self.held
         offsets, starts = self.pages_of.extend(counts)
-        for layer, (k, v) in zip(self.layers, keys_values):
-            append_context(layer.pages, k, v, offsets, starts, self.pages_of.table, positions, rotary_dim)
+        try:
+            for layer, (k, v) in zip(self.layers, keys_values):
+                append_context(layer.pages, k, v, offsets, starts, self.pages_of.table, positions, rotary_dim)
+        except Exception:  # (sizes that the library refuses; what an earlier layer stored lies behind the lengths)
+            self.pages_of._take_back(held)
+            raise
 
     def release(self, context: int) -> None:
         self.pages_of.release(context)

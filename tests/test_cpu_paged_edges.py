@@ -35,3 +35,23 @@ def test_selection_refuses_counts_that_its_index_would_pass(host_only, count):
     with pytest.raises(ValueError, match="below 2"):
         P.select_pages(torch.zeros(1, 1, 40), pages(), ints(1, 2), ints(1), 2, count)
     assert not host_only
+
+
+def test_an_append_that_the_library_refuses_leaves_the_memory_as_it_was(host_only, monkeypatch):
+    m = P.ContextMemory(2, 3, 12, 2, 16, 16, device="cpu")
+    rows = lambda n: [(torch.zeros(n, 32), torch.zeros(n, 32))] * 2  # noqa: E731
+    m.append([17, 0, 3], rows(20))
+    t = m.pages_of
+    before = (t.table.clone(), t.lengths.clone(), m.held, list(t._free), [list(p) for p in t._pages])
+
+    def refused(*args):
+        raise RuntimeError("mmf_paged_append: too many tokens or heads for one call")
+
+    with monkeypatch.context() as patch:
+        patch.setattr(P, "_launch", refused)
+        with pytest.raises(RuntimeError, match="too many"):
+            m.append([16, 40, 1], rows(57))
+    assert torch.equal(t.table, before[0]) and torch.equal(t.lengths, before[1])
+    assert (m.held, t._free, t._pages) == before[2:]
+    m.append([16, 40, 1], rows(57))
+    assert m.held == (33, 40, 4) and len(host_only) == 4
