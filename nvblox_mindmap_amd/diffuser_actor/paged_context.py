@@ -15,6 +15,7 @@ import math
 from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 
@@ -127,12 +128,12 @@ def _check_ints(keys: torch.Tensor, **ts: Tuple[torch.Tensor, int]) -> None:
 def _check_device(index: int, *ts: Optional[torch.Tensor]) -> None:
     if index < 0:
         raise RuntimeError("paged contexts live on an MI355X (no CPU fallback)")
-    grad = torch.is_grad_enabled()
+    grad, tangents = torch.is_grad_enabled(), forward_ad._current_level >= 0
     for t in ts:
         if t is not None:
             if t.get_device() != index:
                 raise ValueError(f"all tensors on cuda:{index}: got one on {t.device}")
-            if grad and t.requires_grad:
+            if (grad and t.requires_grad) or (tangents and forward_ad.unpack_dual(t).tangent is not None):
                 raise RuntimeError("paged contexts have no backward pass: call them under torch.no_grad(), or detach the inputs")
 
 
@@ -162,7 +163,7 @@ def _check_rows(context: ContextPages, k: torch.Tensor, v: torch.Tensor, positio
                 rotary_base: float) -> Tuple[int, int, int, int]:
     """What ``append_context`` asks of the pages and the rows.  -> (rows, axes, rotated channels, address of the positions)"""
     keys, hd = context.keys, context.head_dim
-    _check_device(keys.get_device(), k, v, positions)
+    _check_device(keys.get_device(), k, v, positions, keys, context.values)
     if not _pages_ok(context, True):
         _check_pages(context, True)
     row = keys.shape[1] * hd
@@ -226,7 +227,7 @@ def _check_query(q: torch.Tensor, context: ContextPages, table: torch.Tensor, le
     """What the attention and the selection ask of pages, query and table.  -> (contexts, tokens, slots)"""
     keys = context.keys
     index = keys.get_device()
-    _check_device(index, q)
+    _check_device(index, q, keys, context.values)
     if not _pages_ok(context, summary):
         _check_pages(context, summary)
     h = keys.shape[1]

@@ -80,3 +80,30 @@ def test_lengths_far_outside_the_table(n, dtype):
         assert bool(((got.double() - want).abs() <= bound).all())
     got = P.select_pages(q.cuda(), context, table.cuda(), lengths, 2, 3).cpu()
     assert torch.equal(got, R.select(q, pages[2], pages[3], table, [held], 16, 2, 16, 3))
+
+
+@pytest.mark.parametrize("kind", ["gradient", "tangent"])
+def test_inputs_with_derivatives_are_refused(kind):
+    """No operator loses a gradient or a tangent in silence: of the query, the rows, the positions, or the pages themselves."""
+    from torch.autograd import forward_ad
+
+    def mark(t):
+        return t.clone().requires_grad_() if kind == "gradient" else forward_ad.make_dual(t.clone(), torch.ones_like(t))
+
+    table, lengths, offsets = i32([[0, 1]]).cuda(), i32([20]).cuda(), i32([0, 3]).cuda()
+    q, rows, positions = torch.randn(1, 1, 32).cuda(), torch.randn(3, 32).cuda(), torch.rand(3, 1).cuda()
+    context = P.ContextPages(*(t.cuda() for t in R.make_pages(2, 2, 16, 16, torch.float32)), 16)
+    with forward_ad.dual_level():
+        marked = [context._replace(keys=mark(context.keys)), context._replace(values=mark(context.values))]
+        calls = [lambda: P.context_attention(mark(q), context, table, lengths, 2), lambda: P.select_pages(mark(q), context, table, lengths, 2, 1),
+                 lambda: P.append_context(context, mark(rows), rows, offsets, lengths, table), lambda: P.append_context(context, rows, mark(rows), offsets, lengths, table),
+                 lambda: P.append_context(context, rows, rows, offsets, lengths, table, mark(positions))]
+        calls += [lambda c=c: P.context_attention(q, c, table, lengths, 2) for c in marked]
+        calls += [lambda c=c: P.append_context(c, rows, rows, offsets, lengths, table) for c in marked]
+        for call in calls:
+            with pytest.raises(RuntimeError, match="no backward"):
+                call()
+        assert bool(torch.isfinite(P.context_attention(q, context, table, lengths, 2)).all())
+    with torch.no_grad():
+        if kind == "gradient":
+            assert not P.context_attention(mark(q), context, table, lengths, 2).requires_grad
