@@ -263,7 +263,11 @@ class DiffusionHead(nn.Module):
                              f"{len(self.cross_attn.attn)} cross-attention layers")
         counts = mask.sum(dim=1).tolist()
         tokens, positions = enc["context_feats"][mask], enc["context_pos"][mask].to(torch.float32).contiguous()
-        memory.append(counts, [blk.attn.project_paged(tokens) for blk in self.cross_attn.attn], positions, self.cfg.embedding_dim)
+        keys_values = []
+        for blk, layer in zip(self.cross_attn.attn, memory.layers):  # (under autocast the projections are of a type that the pages need not have)
+            k, v = blk.attn.project_paged(tokens)
+            keys_values.append((k, v) if k.dtype is layer.pages.keys.dtype else (k.float(), v.float()))
+        memory.append(counts, keys_values, positions, self.cfg.embedding_dim)
 
     def time_embeddings(self, timesteps, device):
         """time_mlp(sinusoidal(t)) for a list of timesteps in one batched pass ([T, D]): the time part of the conditioning

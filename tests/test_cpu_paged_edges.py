@@ -55,3 +55,17 @@ def test_an_append_that_the_library_refuses_leaves_the_memory_as_it_was(host_onl
     assert (m.held, t._free, t._pages) == before[2:]
     m.append([16, 40, 1], rows(57))
     assert m.held == (33, 40, 4) and len(host_only) == 4
+
+
+@pytest.mark.parametrize("autocast", [torch.bfloat16, torch.float16, None], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_an_observation_is_remembered_under_autocast(host_only, autocast, dtype):
+    """Projections of either half type go into pages of any type."""
+    from nvblox_mindmap_amd.diffuser_actor import DiffuserActor, DiffuserActorConfig
+
+    model = DiffuserActor(DiffuserActorConfig(data_type="mesh", feature_dim=8), torch.tensor([[-1.0, -1, -1], [1, 1, 1]]))
+    memory = model.new_context_memory(2, 8, 16, dtype, device="cpu")
+    enc = {"context_feats": torch.randn(2, 9, 120), "context_pos": torch.rand(2, 9, 3), "context_mask": torch.rand(2, 9) < 0.7}
+    with torch.no_grad(), torch.autocast("cpu", autocast or torch.bfloat16, enabled=autocast is not None):
+        model.prediction_head.extend_memory(memory, enc)
+    assert memory.held == tuple(enc["context_mask"].sum(1).tolist()) and len(host_only) == 2

@@ -107,3 +107,32 @@ def test_inputs_with_derivatives_are_refused(kind):
     with torch.no_grad():
         if kind == "gradient":
             assert not P.context_attention(mark(q), context, table, lengths, 2).requires_grad
+
+
+def mesh_model(seed=0):
+    from nvblox_mindmap_amd.diffuser_actor import DiffuserActor, DiffuserActorConfig
+
+    torch.manual_seed(seed)
+    model = DiffuserActor(DiffuserActorConfig(data_type="mesh", feature_dim=16, diffusion_timesteps=3), torch.tensor([[-1.0, -1, -1], [1, 1, 1]]))
+    return model.cuda().eval()
+
+
+def mesh_observation(seed, batch=2, n=120):
+    """Arguments of DiffuserActor.forward."""
+    g = torch.Generator().manual_seed(seed)
+    pose = torch.cat([torch.rand(batch, 3, 2, 3, generator=g), torch.nn.functional.normalize(torch.randn(batch, 3, 2, 4, generator=g), dim=-1), torch.ones(batch, 3, 2, 1)], -1)
+    return [None] * 5 + [torch.randn(batch, n, 16, generator=g).cuda(), (torch.rand(batch, n, 3, generator=g) * 1.8 - 0.9).cuda(),
+                         (torch.rand(batch, n, generator=g) > 0.3).cuda(), None, pose.cuda()]
+
+
+@pytest.mark.parametrize("autocast", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@torch.no_grad()
+def test_the_policy_keeps_a_memory_under_autocast(autocast, dtype):
+    model = mesh_model()
+    memory = model.new_context_memory(2, 32, 16, dtype)
+    one, two = mesh_observation(1), mesh_observation(2)
+    with torch.autocast("cuda", autocast):
+        for args in (one, two):
+            assert bool(torch.isfinite(model(*args, run_inference=True, context_memory=memory)[0]).all())
+    assert memory.held == tuple((one[7].sum(1) + two[7].sum(1)).tolist())
