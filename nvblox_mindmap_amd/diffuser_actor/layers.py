@@ -132,6 +132,11 @@ class RelativeAttention(nn.Module):
         kv = self.kv_proj(tokens)
         return kv[:, :self.dim], kv[:, self.dim:]
 
+    def empty_value(self) -> torch.Tensor:
+        """What a query of a context without tokens gets from a ContextMemory: the value of zeroed tokens, which such a sample attends to
+        without one (DiffusionHead.prepare_context)."""
+        return self.kv_proj.bias[self.dim:]
+
     def project_kv_heads(self, memory: torch.Tensor, kv_rot=None):
         """(head-major keys, transposed values, Lk) of a memory for the matrix-core attention kernel (fused inference;
         AttentionStack consumes 3-tuples in ``kv_caches`` this way)."""
@@ -164,7 +169,7 @@ class RelativeAttention(nn.Module):
             q = self.q_proj(query)
             if q_rot is not None:
                 q = apply_rotary(q, *q_rot)
-            return self.out_proj(kv_cache.attend(q, self.heads)), None
+            return self.out_proj(kv_cache.attend(q, self.heads, self.empty_value())), None
         Lk = memory.shape[1]
         if _fused(query) and not need_weights and (D // self.heads) in (8, 15, 16, 20, 24, 32):  # head dims the kernel is built for
             from .fused_ops import attention_small, rotary_apply
@@ -236,7 +241,7 @@ class AttentionBlock(nn.Module):
                 ss = cond_act.lookup(self.adaln) if isinstance(cond_act, AdaLNBatch) else self.adaln.proj(F.silu(cond) if cond_act is None else cond_act)
             q = FO.q_block(query, ss, A.q_proj, q_rot)
             if isinstance(kv_cache, LayerContext):
-                att = kv_cache.attend(q, A.heads)
+                att = kv_cache.attend(q, A.heads, A.empty_value())
             else:
                 k, v = kv_cache if kv_cache is not None else FO.kv_block(memory, A.kv_proj, kv_rot if q_rot is not None else None)
                 att = FO.attention_small(q, k, v, key_padding_mask, A.heads)
@@ -378,7 +383,10 @@ class AttentionStack(nn.Module):
                     q = FO.q_block(query, ss_of(blk.adaln), A.q_proj, q_rot)
                     if not paged:
                         k, v = kv_caches[li] if kv_caches is not None else FO.kv_block(memory, A.kv_proj, kv_rot if q_rot is not None else None)
-                att = kv_caches[li].attend(q, A.heads) if paged and not self.self_attention else FO.attention_small(q, k, v, key_padding_mask, A.heads)
+                if paged and not self.self_attention:
+                    att = kv_caches[li].attend(q, A.heads, A.empty_value())
+                else:
+                    att = FO.attention_small(q, k, v, key_padding_mask, A.heads)
                 query = FO.out_ffn_block(att, query, A.out_proj, blk.norm, ss_of(ffw.adaln), ffw.fc1, ffw.fc2, ffw.norm)
             return query, None
         for li, (attn, ffw) in enumerate(zip(self.attn, self.ffw)):

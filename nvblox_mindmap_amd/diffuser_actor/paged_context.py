@@ -403,13 +403,18 @@ class LayerContext:
     def __init__(self, memory: "ContextMemory", pages: ContextPages):
         self.memory, self.pages = memory, pages
 
-    def attend(self, q: torch.Tensor, heads: int) -> torch.Tensor:
+    def attend(self, q: torch.Tensor, heads: int, empty: Optional[torch.Tensor] = None) -> torch.Tensor:
         """softmax(q k^T / sqrt(head_dim)) v of rotated queries [contexts, T, heads * head_dim] over the memory (over its
-        ``selected_pages`` best pages where that is set); 16-bit pages: q is rounded to their type, the result is of q's."""
+        ``selected_pages`` best pages where that is set); 16-bit pages: q is rounded to their type, the result is of q's.
+        ``empty`` [heads * head_dim]: the result for a context that holds nothing (zeros unless given)."""
         m, t = self.memory, self.memory.pages_of
         x = q if q.dtype is self.pages.keys.dtype else q.to(self.pages.keys.dtype)
         chosen = None if m.selected_pages is None else select_pages(x, self.pages, t.table, t.lengths, heads, m.selected_pages)
-        return context_attention(x, self.pages, t.table, t.lengths, heads, pages=chosen).to(q.dtype)
+        out = context_attention(x, self.pages, t.table, t.lengths, heads, pages=chosen).to(q.dtype)
+        # (the host knows whether there is such a context now; a graph is replayed when there may be)
+        if empty is not None and (0 in t._held or torch.cuda.is_current_stream_capturing()):
+            out = torch.where((t.lengths > 0)[:, None, None], out, empty.to(out.dtype))
+        return out
 
 
 class ContextMemory:

@@ -136,3 +136,55 @@ def test_the_policy_keeps_a_memory_under_autocast(autocast, dtype):
         for args in (one, two):
             assert bool(torch.isfinite(model(*args, run_inference=True, context_memory=memory)[0]).all())
     assert memory.held == tuple((one[7].sum(1) + two[7].sum(1)).tolist())
+
+
+@pytest.mark.parametrize("on", [False, True], ids=["composite", "fused"])
+@torch.no_grad()
+def test_a_robot_that_has_seen_nothing(on):
+    """A sample without a valid context token attends, without a memory, to zeroed tokens, whose values are the projection's bias; a memory
+    that holds nothing of it gives the same."""
+    from nvblox_mindmap_amd.diffuser_actor import DiffuserActor
+
+    model = mesh_model()
+    for name, p in model.named_parameters():  # as a trained model has them
+        if name.endswith("kv_proj.bias"):
+            torch.nn.init.normal_(p, std=0.5)
+        if name.endswith("adaln.proj.weight"):
+            torch.nn.init.normal_(p, std=0.05)
+    args = mesh_observation(5)
+    args[7][1] = False
+    memory = model.new_context_memory(2, 32, 16)
+    DiffuserActor.enable_fused_inference(on)
+    try:
+        torch.manual_seed(3)
+        plain = model(*args, run_inference=True)[0]
+        torch.manual_seed(3)
+        kept = model(*args, run_inference=True, context_memory=memory)[0]
+        # two float32 evaluations of a denoising loop of three steps, positions in metres (as between the two evaluations of a full context)
+        assert float((plain - kept)[..., :3].abs().max()) <= 5e-3
+        stack, query, cond = model.prediction_head.cross_attn, torch.randn(2, 4, 120).cuda(), torch.randn(2, 120).cuda()
+        nothing = torch.zeros(2, 1, 120).cuda()
+        want = stack(query, nothing, cond)[0][1]
+        # 32-bit evaluations of one layer's worth of sums of 120 products, through two layers with a gain of a few each
+        assert float((stack(query, None, cond, kv_caches=memory.layers)[0][1] - want).abs().max()) <= 2e-4
+        # captured: an empty context may have tokens, or lose them, between replays
+        graph = torch.cuda.CUDAGraph()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            stack(query, None, cond, kv_caches=memory.layers)
+        torch.cuda.current_stream().wait_stream(side)
+        with torch.cuda.graph(graph):
+            out = stack(query, None, cond, kv_caches=memory.layers)[0]
+        for step in range(3):
+            if step == 1:
+                memory.release(0)
+            elif step == 2:
+                rows = torch.randn(40, 120).cuda()
+                memory.append([0, 40], [(rows, rows)] * 2)
+            graph.replay()
+            assert torch.equal(out, stack(query, None, cond, kv_caches=memory.layers)[0]), step
+            if step == 1:
+                assert float((out - stack(query, nothing, cond)[0]).abs().max()) <= 2e-4
+    finally:
+        DiffuserActor.enable_fused_inference(False)
