@@ -598,8 +598,9 @@ int mmf_paged_width(int head_dim);
  * offsets[B] are not read; tokens beyond the table are not stored.  rotary_dim != 0: the keys' channel pairs (2 i, 2 i + 1) are rotated
  * on the way by positions [tokens, axes] (float32): the first rotary_dim channels of every head, or of the whole row if rotary_dim ==
  * kv_heads * head_dim; axis a has the channels [a, a + 1) * rotary_dim / axes, pair j of it turns by position_a * rotary_base^(-2 j axes /
- * rotary_dim) -- with axes = 3 and the whole row the policy's code (mindmap/diffuser_actor/position_encodings.py).  Keys are rounded once
- * to the pages' type; a page's key_min / key_max begin anew with the token in its first slot. */
+ * rotary_dim), rotary_base positive and finite -- with axes = 3 and the whole row the policy's code
+ * (mindmap/diffuser_actor/position_encodings.py).  Keys are rounded once to the pages' type; a page's key_min / key_max begin anew with the
+ * token in its first slot. */
 int mmf_paged_append(const void* k_dev, int64_t k_row_stride, const void* v_dev, int64_t v_row_stride, int in_type, int64_t tokens,
                      const float* positions_dev, int axes, int rotary_dim, double rotary_base, const int32_t* offsets_dev,
                      const int32_t* starts_dev, const int32_t* table_dev, int B, int slots, int page_size, int kv_heads, int head_dim,

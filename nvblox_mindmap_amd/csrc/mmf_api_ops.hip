@@ -601,8 +601,8 @@ int mmf_paged_append(const void* k, int64_t k_row_stride, const void* v, int64_t
   const int64_t row = (int64_t)kv_heads * head_dim;
   if (row > 0x7fffffffLL) return paged_fail(name, "kv_heads * head_dim passes 31 bits");
   if (rotary_dim) {
-    if (!positions || axes < 1 || axes > 4 || rotary_dim < 0 || rotary_dim % (2 * axes) || (rotary_dim > head_dim && rotary_dim != row) || !(rotary_base > 0))
-      return paged_fail(name, "rotary_dim is a multiple of 2 * axes, at most head_dim or kv_heads * head_dim, with positions of 1 to 4 axes");
+    if (!positions || axes < 1 || axes > 4 || rotary_dim < 0 || rotary_dim % (2 * axes) || (rotary_dim > head_dim && rotary_dim != row) || !(rotary_base > 0) || rotary_base == HUGE_VAL)
+      return paged_fail(name, "rotary_dim is a multiple of 2 * axes, at most head_dim or kv_heads * head_dim, with positions of 1 to 4 axes and a positive, finite base");
   }
   if (tokens == 0) return MMF_OK;
   if (!k || !v || k_row_stride < 0 || v_row_stride < 0 || k_row_stride >= (1 << 23) || v_row_stride >= (1 << 23))

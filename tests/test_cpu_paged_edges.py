@@ -69,3 +69,10 @@ def test_an_observation_is_remembered_under_autocast(host_only, autocast, dtype)
     with torch.no_grad(), torch.autocast("cpu", autocast or torch.bfloat16, enabled=autocast is not None):
         model.prediction_head.extend_memory(memory, enc)
     assert memory.held == tuple(enc["context_mask"].sum(1).tolist()) and len(host_only) == 2
+
+
+@pytest.mark.parametrize("base", [float("inf"), float("nan"), -1.0])
+def test_the_c_append_refuses_a_rotary_base_without_angles(base):
+    fake = C.c_void_p(4096)
+    rc = _lib.lib().mmf_paged_append(fake, 40, fake, 40, 0, 3, fake, 1, 20, base, fake, fake, fake, 1, 2, 16, 2, 20, 4, 0, fake, fake, fake, fake, None)
+    assert rc != 0 and "positive, finite base" in _lib.last_error()
