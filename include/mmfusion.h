@@ -587,7 +587,7 @@ int mmf_attention_small(const float* q_dev, const float* k_dev, long long k_row_
  *                              beginning) as long as one call's tokens go to it from one context only.
  *   lengths [B] int32          tokens a context holds; clamped to [0, slots * page_size]
  * W = mmf_paged_width(head_dim): head_dim rounded up to 16, 32, 64, 96, 128 or 256; the channels behind head_dim are zero (allocate them
- * so; an append writes zeros there at most).  page_size 16, 32, 64, 128 or 256.  Pools aligned to 16 bytes.  All sizes that depend on the device data
+ * so; an append writes zeros there at most).  page_size 16, 32, 64, 128 or 256.  Pools and workspaces aligned to 16 bytes.  All sizes that depend on the device data
  * (lengths, offsets, tables) are read on the device: a captured graph replays with new ones. */
 #define MMF_TYPE_F32 0
 #define MMF_TYPE_F16 1

@@ -1,6 +1,7 @@
 // mmf_api_ops.hip -- the stateless entry points of the C ABI (include/mmfusion.h): depth back-projection, mask algebra, feature
 // resize and the policy-side ops (farthest-point sampling, the fused inference kernels).
 #include <chrono>
+#include <initializer_list>
 #include <mutex>
 
 #include "mmf_api_internal.h"
@@ -585,6 +586,13 @@ const char* paged_shape_error(int type, int B, int slots, int page_size, int H, 
   if ((int64_t)H * page_size * paged_width(head_dim) > (1 << 30)) return "a page passes 2^30 elements";
   return nullptr;
 }
+// the kernels move pages and partial results in pieces of 16 bytes
+bool unaligned16(std::initializer_list<const void*> ps) {
+  uintptr_t any = 0;
+  for (const void* p : ps) any |= (uintptr_t)p;
+  return (any & 15) != 0;
+}
+const char* const kUnaligned = "pools and workspace are aligned to 16 bytes";
 int page_shift(int page_size) { return __builtin_ctz((unsigned)page_size); }
 int paged_fail(const char* name, const char* why) { return fail(MMF_ERR_INVALID_ARG, std::string(name) + ": " + why); }
 }  // namespace
@@ -598,6 +606,7 @@ int mmf_paged_append(const void* k, int64_t k_row_stride, const void* v, int64_t
   if (tokens < 0 || tokens > 0x7fffffffLL) return paged_fail(name, "0 <= tokens < 2^31");
   if (in_type != type && in_type != MMF_TYPE_F32) return paged_fail(name, "k and v are of the pages' type or float32");
   if (!offsets || !starts || !table || !keys || !values || !key_min || !key_max) return paged_fail(name, "null pointer");
+  if (unaligned16({keys, values, key_min, key_max})) return paged_fail(name, kUnaligned);
   const int64_t row = (int64_t)kv_heads * head_dim;
   if (row > 0x7fffffffLL) return paged_fail(name, "kv_heads * head_dim passes 31 bits");
   if (rotary_dim) {
@@ -625,6 +634,7 @@ int mmf_paged_attention(const void* q, const void* keys, const void* values, int
   const char* name = "mmf_paged_attention";
   if (const char* e = paged_shape_error(type, B, slots, page_size, kv_heads, head_dim, num_pages)) return paged_fail(name, e);
   if (!q || !keys || !values || !table || !lengths || !out) return paged_fail(name, "null pointer");
+  if (unaligned16({keys, values, workspace})) return paged_fail(name, kUnaligned);
   if (T <= 0 || group <= 0 || (int64_t)T * group > (1 << 24) || (int64_t)kv_heads * group * head_dim > 0x7fffffffLL)
     return paged_fail(name, "positive T and group");
   if (selected && (count <= 0 || (int64_t)count * page_size > (1 << 30))) return paged_fail(name, "count > 0, count * page_size up to 2^30");
@@ -646,6 +656,7 @@ int mmf_paged_select(const void* q, const void* key_min, const void* key_max, in
   const char* name = "mmf_paged_select";
   if (const char* e = paged_shape_error(type, B, slots, page_size, kv_heads, head_dim, num_pages)) return paged_fail(name, e);
   if (!q || !key_min || !key_max || !table || !lengths || !selected || !workspace) return paged_fail(name, "null pointer");
+  if (unaligned16({key_min, key_max, workspace})) return paged_fail(name, kUnaligned);
   if (T <= 0 || group <= 0 || count <= 0 || (int64_t)kv_heads * group * head_dim > 0x7fffffffLL) return paged_fail(name, "positive T, group and count");
   if (count >= (1 << 30)) return paged_fail(name, "count is below 2^30");
   if (workspace_bytes < mmf_paged_select_workspace_bytes(B, T, kv_heads, slots)) return paged_fail(name, "workspace smaller than mmf_paged_select_workspace_bytes");

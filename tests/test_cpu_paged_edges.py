@@ -76,3 +76,17 @@ def test_the_c_append_refuses_a_rotary_base_without_angles(base):
     fake = C.c_void_p(4096)
     rc = _lib.lib().mmf_paged_append(fake, 40, fake, 40, 0, 3, fake, 1, 20, base, fake, fake, fake, 1, 2, 16, 2, 20, 4, 0, fake, fake, fake, fake, None)
     assert rc != 0 and "positive, finite base" in _lib.last_error()
+
+
+@pytest.mark.parametrize("entry,args", [("append", (0, 1, 2, 3)), ("attention", (0, 1, 2)), ("select", (0, 1, 2))])
+def test_the_c_entries_refuse_unaligned_pools_and_workspaces(entry, args):
+    fake, odd = C.c_void_p(4096), C.c_void_p(4104)
+    for bad in args:
+        p = [odd if i == bad else fake for i in range(4)]
+        if entry == "append":
+            rc = _lib.lib().mmf_paged_append(fake, 40, fake, 40, 0, 3, fake, 1, 20, 100.0, fake, fake, fake, 1, 2, 16, 2, 20, 4, 0, *p, None)
+        elif entry == "attention":
+            rc = _lib.lib().mmf_paged_attention(fake, p[0], p[1], 0, fake, fake, None, 0, 2, 1, 2, 1, 20, 100, 4, 256, 1.0, fake, p[2], 1 << 40, None)
+        else:
+            rc = _lib.lib().mmf_paged_select(fake, p[0], p[1], 0, fake, fake, 2, 1, 2, 1, 20, 100, 4, 16, 3, fake, p[2], 1 << 30, None)
+        assert rc != 0 and "aligned to 16 bytes" in _lib.last_error()
