@@ -188,3 +188,98 @@ def test_a_robot_that_has_seen_nothing(on):
                 assert float((out - stack(query, nothing, cond)[0]).abs().max()) <= 2e-4
     finally:
         DiffuserActor.enable_fused_inference(False)
+
+
+# ---- launch forms of large calls ----
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("hd", [15, 80, 128, 250])  # widths 16, 96, 128, 256
+@pytest.mark.parametrize("rows,n", [(17, 5003), (33, 3001), (40, 4099), (17, 20005), (33, 18000)])  # at most 64 splits, and more
+def test_many_rows_over_split_contexts(dtype, hd, rows, n):
+    """17 and more query rows of a key-value head -- two row tiles, several row blocks -- whose partial results are joined; as query tokens, as
+    heads that share the keys, and as such heads over selected pages."""
+    page, g = 256, torch.Generator().manual_seed(rows + n)
+    need = -(-n // page)
+    pages = R.make_pages(need, 1, page, hd, dtype, n)
+    table = R.make_table([need], need + 1, need, n)
+    context, lengths = P.ContextPages(*(t.cuda() for t in pages), hd), i32([n]).cuda()
+    at = table[0, :need].long()
+    k = pages[0][at, 0, :, :hd].reshape(-1, hd)[:n].double()
+    v = pages[1][at, 0, :hd].permute(0, 2, 1).reshape(-1, hd)[:n].double()
+    x = (1.5 * torch.randn(rows, hd, generator=g)).to(dtype)
+    slots = torch.randperm(need + 1, generator=g)[:need - 2].to(torch.int32)  # (the last slot of the table has no page)
+    place = torch.arange(n) // page
+    for q, heads, chosen in ((x.view(1, rows, hd), 1, None), (x.view(1, 1, rows * hd), rows, None), (x.view(1, 1, rows * hd), rows, slots)):
+        kk, vv = (k, v) if chosen is None else (k[torch.isin(place, chosen.long())], v[torch.isin(place, chosen.long())])
+        got = P.context_attention(q.cuda(), context, table.cuda(), lengths, heads, pages=None if chosen is None else chosen.view(1, 1, 1, -1).cuda()).cpu()
+        xd = x.double()
+        p = torch.softmax(xd @ kk.T * hd ** -0.5, 1)
+        want, size = p @ vv, (xd.abs() @ kk.abs().T).amax(1, keepdim=True) * hd ** -0.5
+        # the bound of paged_reference.attention
+        rel = 2 * (hd + 4) * R.U * size + (len(kk) + 8) * R.U + (0.0 if dtype == torch.float32 else 2.0 ** -16 + len(kk) * 2.0 ** -31)
+        bound = 2 * rel * (p @ vv.abs()) + R.HALF_STEP[dtype] * want.abs() * (1 + rel) + 2.0 ** -25 * (dtype == torch.float16)
+        off = (got.view(rows, hd).double() - want).abs()
+        assert bool((off <= bound).all()), (heads, chosen is not None, float((off / bound).max()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("hd,batch,kv,slots", [(250, 8, 16, 531), (128, 8, 16, 1060), (80, 16, 16, 530), (64, 16, 12, 1400), (16, 16, 16, 4100), (128, 16, 16, 8200)])
+@pytest.mark.parametrize("tokens,group", [(1, 1), (2, 4), (3, 3), (1, 17)])
+def test_scores_of_many_pages(dtype, hd, batch, kv, slots, tokens, group):
+    """Workgroups that score several sets of pages one after the other (up to 16), with eight query rows a key-value head and with more; the
+    same pages stand in many slots, so equal scores abound."""
+    pool, page, count, g = 96, 16, 9, torch.Generator().manual_seed(hd + slots)
+    pages = R.make_pages(pool, kv, page, hd, dtype, hd)
+    table = torch.randint(-1, pool, (batch, slots), generator=g).to(torch.int32)
+    held = torch.randint(1, slots + 1, (batch,), generator=g)
+    held[0], held[1] = slots, 0
+    q = torch.randn(batch, tokens, kv * group * hd, generator=g).to(dtype)
+    got = P.select_pages(q.cuda(), P.ContextPages(*(t.cuda() for t in pages), hd), table.cuda(), (held * page).to(torch.int32).cuda(), kv * group, count).cpu()
+    x = q.double().view(batch, tokens, kv, group, hd).permute(2, 0, 1, 3, 4).reshape(kv, -1, hd)
+    low, high = (t[..., :hd].double().permute(1, 2, 0).contiguous() for t in (pages[2], pages[3]))
+    score = (torch.matmul(x.clamp(min=0), high) + torch.matmul(x.clamp(max=0), low)).view(kv, batch, tokens, group, pool).amax(3)
+    for b in range(batch):
+        there = (torch.arange(slots) < held[b]) & (table[b] >= 0)
+        s = score[:, b][..., table[b].clamp(min=0).long()].masked_fill(~there, -math.inf)  # [kv, tokens, slots]
+        order = torch.sort(s, dim=-1, descending=True, stable=True).indices[..., :count]
+        order = torch.where(torch.gather(s, 2, order) > -math.inf, order, slots).sort(-1).values
+        want = torch.where(order < slots, order, -1).to(torch.int32)
+        assert torch.equal(got[b], want.transpose(0, 1)), b
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("selected", [None, 2])
+@torch.no_grad()
+def test_a_memory_in_16_bits_is_that_of_its_rounded_keys_and_values(dtype, selected):
+    """Two observations through the policy's projections: the pages hold them rounded once, and a layer's attention is that of the rounded
+    query over them."""
+    head = mesh_model(1).prediction_head
+    memory = P.ContextMemory(2, 2, 16, 8, 15, 16, dtype, selected_pages=selected)
+    g, seen = torch.Generator().manual_seed(7), [[], []]
+    for sizes in ((40, 7), (23, 30)):
+        n = max(sizes)
+        mask = torch.arange(n)[None] < torch.tensor(sizes)[:, None]
+        enc = {"context_feats": torch.randn(2, n, 120, generator=g).cuda(), "context_pos": (torch.rand(2, n, 3, generator=g) * 2 - 1).cuda(), "context_mask": mask.cuda()}
+        head.extend_memory(memory, enc)
+        for b, m in enumerate(sizes):
+            seen[b].append((enc["context_feats"][b, :m], enc["context_pos"][b, :m].cpu()))
+    t = memory.pages_of
+    assert t.held == (63, 37)
+    for layer, blk in zip(memory.layers, head.cross_attn.attn):
+        pages = [x.cpu() for x in layer.pages[:4]]
+        for b in range(2):
+            for h in range(8):
+                k, v, _ = R.context(pages, t.table[b].cpu(), t.held[b], h, 15)
+                start = 0
+                for f, xyz in seen[b]:
+                    kv = blk.attn.kv_proj(f).cpu().double()
+                    rotated = R.rotate(kv[:, :120], xyz, None, 8, 15)[:, 15 * h:15 * h + 15]
+                    for got, want in ((k, rotated), (v, kv[:, 120 + 15 * h:135 + 15 * h])):
+                        # the rounding to the pages' type; rotation in 32 bits, and the projection of more rows at once: sums of 120 products in another order
+                        slack = (12 * 2 + 2 * 120) * R.U * float(kv.abs().max()) * 2 + 2.0 ** -25 * (dtype == torch.float16)
+                        assert bool(((got[start:start + len(f)] - want).abs() <= R.HALF_STEP[dtype] * want.abs() + slack).all())
+                    start += len(f)
+        q = torch.randn(2, 3, 120, generator=g)
+        chosen = None if selected is None else R.select(q.to(dtype), pages[2], pages[3], t.table.cpu(), t.held, 16, 8, 15, selected)
+        want, bound = R.attention(q.to(dtype), pages, t.table.cpu(), t.held, 8, 15, selected=chosen)
+        got = layer.attend(q.cuda(), 8, blk.attn.empty_value())
+        assert got.dtype == torch.float32 and bool(((got.cpu().double() - want).abs() <= bound).all())
