@@ -7,7 +7,9 @@
 //   * reciprocal: EXHAUSTIVELY, every float32 in [2^lo, 2^hi) -- enumeration is the proof;
 //   * quotient a / b (Markstein: y = RN(1/b), q = RN(a y), r = a - b q exactly, q' = RN(q + r y)): a theorem given y, checked
 //     here on 2^36 random pairs as a guard against a slip in the restatement.
-// Build + run (GPU box):  hipcc --offload-arch=gfx950 -O3 -ffp-contract=off tools/microbench/exact_division.hip -o /tmp/exdiv && /tmp/exdiv
+// Build + run (no packed float32 instructions, as in the library's Makefile):
+//   hipcc --offload-arch=gfx950 -O3 -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops tools/microbench/exact_division.hip -o /tmp/exdiv
+//   /tmp/exdiv
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

@@ -1,5 +1,6 @@
 // Wave / workgroup dispatch rate of the device: duration of kernels that do (almost) nothing, as a function of the
-// number of workgroups and the workgroup size.  hipcc --offload-arch=gfx950 -O2 -o wave_rate tools/wave_rate.hip
+// number of workgroups and the workgroup size.
+//   hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops -o wave_rate tools/wave_rate.hip
 #include <hip/hip_runtime.h>
 
 #include <cstdio>
