@@ -125,16 +125,25 @@ def _check_ints(keys: torch.Tensor, **ts: Tuple[torch.Tensor, int]) -> None:
         _check(_ints_ok(t, dim, keys.get_device()), f"{name}: a contiguous int32 tensor of {dim} dimension(s) on {keys.device}")
 
 
-def _check_device(index: int, *ts: Optional[torch.Tensor]) -> None:
+def _no_backward() -> RuntimeError:
+    return RuntimeError("paged contexts have no backward pass: call them under torch.no_grad(), or detach the inputs")
+
+
+def _check_device(index: int, keys: torch.Tensor, values: torch.Tensor, *ts: Optional[torch.Tensor]) -> None:
+    """The inputs ``ts`` on the pages' device; no derivative in them or in the pages (whose devices _pages_ok compares)."""
     if index < 0:
         raise RuntimeError("paged contexts live on an MI355X (no CPU fallback)")
-    grad, tangents = torch.is_grad_enabled(), forward_ad._current_level >= 0
+    grad = torch.is_grad_enabled()
     for t in ts:
         if t is not None:
             if t.get_device() != index:
                 raise ValueError(f"all tensors on cuda:{index}: got one on {t.device}")
-            if (grad and t.requires_grad) or (tangents and forward_ad.unpack_dual(t).tangent is not None):
-                raise RuntimeError("paged contexts have no backward pass: call them under torch.no_grad(), or detach the inputs")
+            if grad and t.requires_grad:
+                raise _no_backward()
+    if grad and (keys.requires_grad or values.requires_grad):
+        raise _no_backward()
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (keys, values, *ts)):
+        raise _no_backward()
 
 
 def _launch(index: int, entry, what: str, *args) -> None:
@@ -163,7 +172,7 @@ def _check_rows(context: ContextPages, k: torch.Tensor, v: torch.Tensor, positio
                 rotary_base: float) -> Tuple[int, int, int, int]:
     """What ``append_context`` asks of the pages and the rows.  -> (rows, axes, rotated channels, address of the positions)"""
     keys, hd = context.keys, context.head_dim
-    _check_device(keys.get_device(), k, v, positions, keys, context.values)
+    _check_device(keys.get_device(), keys, context.values, k, v, positions)
     if not _pages_ok(context, True):
         _check_pages(context, True)
     row = keys.shape[1] * hd
@@ -227,7 +236,7 @@ def _check_query(q: torch.Tensor, context: ContextPages, table: torch.Tensor, le
     """What the attention and the selection ask of pages, query and table.  -> (contexts, tokens, slots)"""
     keys = context.keys
     index = keys.get_device()
-    _check_device(index, q, keys, context.values)
+    _check_device(index, keys, context.values, q)
     if not _pages_ok(context, summary):
         _check_pages(context, summary)
     h = keys.shape[1]
