@@ -587,8 +587,8 @@ int mmf_attention_small(const float* q_dev, const float* k_dev, long long k_row_
  *                              beginning) as long as one call's tokens go to it from one context only.
  *   lengths [B] int32          tokens a context holds; clamped to [0, slots * page_size]
  * W = mmf_paged_width(head_dim): head_dim rounded up to 16, 32, 64, 96, 128 or 256; the channels behind head_dim are zero (allocate them
- * so; an append writes zeros there at most).  page_size 16, 32, 64, 128 or 256.  Pools and workspaces aligned to 16 bytes.  All sizes that depend on the device data
- * (lengths, offsets, tables) are read on the device: a captured graph replays with new ones. */
+ * so; an append writes zeros there at most).  page_size 16, 32, 64, 128 or 256.  Pools and workspaces aligned to 16 bytes.  All sizes that
+ * depend on the device data (lengths, offsets, tables) are read on the device: a captured graph replays with new ones. */
 #define MMF_TYPE_F32 0
 #define MMF_TYPE_F16 1
 #define MMF_TYPE_BF16 2
@@ -608,6 +608,9 @@ int mmf_paged_append(const void* k_dev, int64_t k_row_stride, const void* v_dev,
 /* out = softmax(scale q k^T) v of T query tokens per context over all its tokens: q, out [B, T, kv_heads * group * head_dim] of the pages'
  * type; query head h reads key-value head h / group.  selected != null ([B, T, kv_heads, count] int32, table slots): over the tokens of
  * these slots only (each at most once; an entry outside [0, slots) holds nothing).  No token: zeros.  Statistics and sums in 32 bits.
+ * What lies behind the lengths may be anything; an infinite value among the tokens may give NaN in its channel where the pages have 16 bits (a
+ * weight is then two numbers, the second of which may be zero or negative).  32 query rows (T * group; 16 of more than 128 channels) share
+ * one pass over keys and values.
  * The keys of a context are split over workgroups and joined by a second launch; workspace: mmf_paged_attention_workspace_bytes(...,
  * capacity = (selected ? count : slots) * page_size, selected != 0) bytes, free again when the work is done. */
 int64_t mmf_paged_attention_workspace_bytes(int B, int T, int kv_heads, int group, int head_dim, int64_t capacity, int selected);
@@ -618,7 +621,8 @@ int mmf_paged_attention(const void* q_dev, const void* keys_dev, const void* val
 /* The `count` table slots of every query token and key-value head with the highest scores, ascending, filled up with -1: selected
  * [B, T, kv_heads, count].  A page's score is sum_c max(q_c, 0) key_max_c + min(q_c, 0) key_min_c -- no key of the page has a larger
  * product with q --, the largest over the `group` query heads; in 64 bits, the lower slot first among equals.  A page whose score is not
- * a number comes first.  0 < count < 2^30.  workspace: mmf_paged_select_workspace_bytes bytes. */
+ * a number (a NaN key, an infinite one times a zero) comes first.  The work follows `slots`, the table's width, more than the lengths: a table
+ * as wide as a pool that many contexts share makes rows of the pool's length.  0 < count < 2^30.  workspace: mmf_paged_select_workspace_bytes bytes. */
 int64_t mmf_paged_select_workspace_bytes(int B, int T, int kv_heads, int slots);
 int mmf_paged_select(const void* q_dev, const void* key_min_dev, const void* key_max_dev, int type, const int32_t* table_dev,
                      const int32_t* lengths_dev, int B, int T, int kv_heads, int group, int head_dim, int slots, int num_pages, int page_size,

@@ -53,8 +53,11 @@ __device__ __forceinline__ float larger(float a, float b) { return __builtin_ele
 // Token i of the rows offsets[b] .. offsets[b + 1] - 1 becomes token starts[b] + i - offsets[b] of context b.  A workgroup owns one
 // (context, page) pair and a range of heads, so a page's summary has one writer and needs no atomics; it finds its pair by a scan over
 // the contexts' page counts.  A thread takes VEC channels of VT neighbouring slots: the keys go out row by row as they came, the values
-// are transposed in its registers so that both stores are wide.  Large appends are bound by memory: 138 us for 145 000 tokens of 8 heads of 64
-// (float16, 599 MB: 4.3 TB/s), 39 us for 55 000 of 8 heads of 15 (float32, 107 MB); single tokens by the chain offsets, page, angles, store: 6 us.
+// are transposed in its registers so that both stores are wide.  Large appends of whole 16-byte heads are bound by memory: 138 us for 145 000
+// tokens of 8 heads of 64 (float16, 599 MB: 4.3 TB/s).  Heads of 15 are not: 40 us for 55 000 tokens of 8 of them (float32, 107 MB, all of it moved
+// once), where 120 of 256 threads have a chunk and a page's rows are asked for behind offsets, table entry, positions and angles.  Single tokens are
+// bound by that chain (6 us), those of many contexts by it and by their values: 2 bytes each, every one in a 32-byte piece of its own (12 us for 256
+// contexts of 8 heads of 128: 262 144 such pieces).
 struct AppendArgs {
   const void *k, *v;
   long long k_stride, v_stride;  // below 2^23
@@ -346,8 +349,11 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
 // matrix cores without a pass through LDS: S^T = K Q^T leaves lane group g of a tile with the scores of its keys, which are the operand
 // that O^T = V^T P^T takes from that lane group -- the rows of K are dealt out so that they are 8 neighbouring keys (4 in 32-bit pages), i.e. one
 // 16-byte load of a value row.  What bounds it is the single pass over keys and values:
-// 237 us for 64 contexts of up to 8191 tokens, 8 heads of 128 shared by 32 (1.2 GB: 5.1 TB/s), 732 us for one of 1 000 003 (4.1 GB: 5.6 TB/s); short
-// contexts by the chain length, page, keys, values and the join: 6 + 4 us for 3080 tokens of 8 heads of 15.
+// 240 us for 64 contexts of up to 8191 tokens, 8 heads of 128 shared by 32 (1.2 GB: 5.0 TB/s), 741 us for one of 1 000 003 (4.1 GB: 5.5 TB/s); short
+// contexts by the chain length, page, keys, values and the join: 6 + 4 us for 3080 tokens of 8 heads of 15.  A wave asks for a tile, waits and
+// works, so a launch of few workgroups waits most of its time: 15.5 us for 56 MB of selected pages (336 workgroups, 32-bit).  A pass serves 32
+// query rows of a key-value head (16 of 256 channels): more of them read keys and values again (226 us for 16 tokens, 241 for 32, 318 for 33,
+// 32 contexts of up to 20 011 tokens, 12 heads of 64, float16).
 struct AttArgs {
   const void *q, *keys, *values;
   const int *table, *lengths, *selected;
@@ -496,7 +502,8 @@ __global__ __launch_bounds__(256) void k_paged_attention(AttArgs a) {
       // this lane's key row and value group; a group of 8 (4) keys lies in one page
       f32x4 s[RT][2];
       int left[2];  // valid keys of the lane's score group(s)
-      // the values' loads go out with the keys', where there are registers for both
+      // the values' loads go out with the keys', where there are registers for both (in 32-bit pages with the first 16 keys'; the other 16
+      // are asked for once those are multiplied)
       uint4 early[EARLY ? NV : 1];
       if constexpr (EARLY) {
 #pragma unroll
@@ -824,9 +831,11 @@ struct SelectArgs {
 
 // One summary is read once: W / 8 lanes take 8 channels of a page each, 64 / that many pages side by side in a wave, two such sets at a
 // time as 64-bit numbers in registers, all query rows over them.  The lanes' sums meet in a rotation within the 16-lane row, whose result
-// is the same in every lane.  What bounds it is half the read, half the 64-bit arithmetic (31 us for 76 MB, 4 rows of 128 channels).  Tried
-// and left: the 64-bit matrix instruction (42 TFLOP/s, and it pays for 16 rows whatever their number); 32-bit scores of all pages with a bound on
-// their error and 64-bit ones near the border alone (26 us here, but 5 to 7 more in the selection, and 7 more where rows are short).
+// is the same in every lane.  What bounds it: a step waits for its summaries before its sums begin -- only the table entries of the next are
+// fetched ahead --, so read and work add up (31 us for 76 MB, 4 rows of 128 channels; the read alone is 15 us at a copy's rate, the 64-bit
+// multiplications 4 at the card's).  Tried and left: the 64-bit matrix instruction (42 TFLOP/s, and it pays for 16 rows whatever their
+// number); 32-bit scores of all pages with a bound on their error and 64-bit ones near the border alone (26 us here, but 5 to 7 more in the
+// selection, and 7 more where rows are short).
 template <int N>
 __device__ __forceinline__ double row_rotate(double x) {  // the value N lanes on in the row of 16
   const long long u = __double_as_longlong(x);
@@ -863,7 +872,8 @@ __global__ __launch_bounds__(256) void k_paged_score(SelectArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lc = lane % L, c0 = lc * 8, gp = lane / L;
   const int per_block = 4 * STEP * a.score_steps;
   const int rows = a.T * a.G;
-  // what does not depend on the context's length is asked for together with it: the first step's table entries, the query
+  // what does not depend on the context's length is asked for before it: the first step's table entries, then the query, whose loads each
+  // stand under a condition of their own and wait one for the other (four for heads of 128)
   auto entries = [&](int first, int (&page)[NP]) {
 #pragma unroll
     for (int i = 0; i < NP; ++i) page[i] = a.table[(long long)b * a.slots + min(first + i * GP + gp, a.slots - 1)];

@@ -203,7 +203,8 @@ def append_context(context: ContextPages, k: torch.Tensor, v: torch.Tensor, offs
     tokens ``starts[b]``, ``starts[b] + 1``, ... of context b, in the pages ``table[b]`` [contexts, slots] names; rows behind
     ``offsets[-1]``, and tokens whose table entry is outside [0, num_pages) or behind the table, are not stored.
 
-    With ``positions`` [n, axes] (float32, 1 to 4 axes) the keys are rotated on the way as ``layers.rotary3d`` / ``apply_rotary`` do:
+    With ``positions`` [n, axes] (float32, 1 to 4 axes) the keys are rotated on the way as ``layers.rotary3d`` / ``apply_rotary`` do (pairs
+    of neighbouring channels, 2 i with 2 i + 1; a rotation of a head's halves is not offered):
     ``rotary_dim`` channels, each axis a share of them.  rotary_dim = kv_heads * head_dim (the default): one code over the whole row, the
     policy's; rotary_dim <= head_dim: the first channels of every head.  Angles are taken in 64 bits (far positions keep their fraction).
 
@@ -263,7 +264,8 @@ def context_attention(q: torch.Tensor, context: ContextPages, table: torch.Tenso
     """softmax(scale q k^T) v per head over the first ``lengths[b]`` tokens of context b (scale: 1 / sqrt(head_dim) unless given); q
     [contexts, T, heads * head_dim] of the pages' type, rotated by the caller (``fused_ops.rotary_apply``, ``q_block``); query head i reads
     key-value head i // (heads / kv_heads).  ``pages`` [contexts, T, kv_heads, count] int32 (``select_pages``): over the tokens of these
-    table slots only; an entry outside the table holds nothing, none may stand twice.  Zeros where there is no token.  -> [contexts, T, heads * head_dim]."""
+    table slots only; an entry outside the table holds nothing, none may stand twice.  Zeros where there is no token.  -> [contexts, T, heads * head_dim].
+    A pass over keys and values serves 32 query rows of a key-value head (T * heads / kv_heads; 16 where head_dim > 128): meant for few tokens."""
     b, t, slots = _check_query(q, context, table, lengths, heads, False)
     keys, values, _, _, hd = context
     index = keys.get_device()
@@ -295,7 +297,8 @@ def select_pages(q: torch.Tensor, context: ContextPages, table: torch.Tensor, le
     """Table slots of the ``count`` pages that can hold the largest products with each query token, for every key-value head:
     [contexts, T, kv_heads, count] int32, ascending, filled up with -1 -- the ``pages`` of ``context_attention``.  A page's score is
     sum_c max(q_c, 0) key_max_c + min(q_c, 0) key_min_c, which no key of the page exceeds, the largest over the query heads that share the
-    key-value head; taken in 64 bits, the lower slot first among equals."""
+    key-value head; taken in 64 bits, the lower slot first among equals.  Time and workspace (8 bytes a slot, token and key-value head) follow
+    the table's width, whatever the lengths."""
     b, t, slots = _check_query(q, context, table, lengths, heads, True)
     keys, _, low, high, hd = context
     index = keys.get_device()
@@ -318,7 +321,8 @@ def select_pages(q: torch.Tensor, context: ContextPages, table: torch.Tensor, le
 
 class PageTable:
     """Which pages of a pool belong to which context: the bookkeeping on the host, ``table`` [contexts, slots] and ``lengths`` [contexts] int32
-    on the device, changed in place (a captured graph reads the new ones).  A page belongs to one context."""
+    on the device, changed in place (a captured graph reads the new ones).  A page belongs to one context.  ``slots``: the most pages of a
+    context, all of the pool unless given -- give its share where many contexts share a pool and pages are selected (``select_pages``)."""
 
     def __init__(self, contexts: int, num_pages: int, page_size: int, slots: Optional[int] = None, device="cuda"):
         if contexts < 1 or num_pages < 1 or page_size not in PAGE_SIZES:
