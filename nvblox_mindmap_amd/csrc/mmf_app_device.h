@@ -341,7 +341,7 @@ __device__ __forceinline__ void feature_voxel(const AppArgs& Aa, const MapConsts
           const float4 q00 = reinterpret_cast<const float4*>(p00 + c0)[h], q01 = reinterpret_cast<const float4*>(p01 + c0)[h];
           const float4 q10 = reinterpret_cast<const float4*>(p10 + c0)[h], q11 = reinterpret_cast<const float4*>(p11 + c0)[h];
 #pragma unroll
-          for (int k = 0; k < 4; k += 2) {  // channel pairs: packed f32 multiplies / adds, the arithmetic of low_tap element by element
+          for (int k = 0; k < 4; k += 2) {  // channel pairs: the arithmetic of low_tap element by element
             const f32x2 a = {f4_at(q00, k), f4_at(q00, k + 1)}, b = {f4_at(q01, k), f4_at(q01, k + 1)};
             const f32x2 c = {f4_at(q10, k), f4_at(q10, k + 1)}, d = {f4_at(q11, k), f4_at(q11, k + 1)};
             const f32x2 r0x0 = pk_madd2<FMA>(X0.l0, a, X0.l1, b), r0x1 = pk_madd2<FMA>(X1.l0, a, X1.l1, b);  // upper texel row at the two tap columns
